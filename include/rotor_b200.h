@@ -412,6 +412,71 @@ int rotor_b200_bias_attention(const rotor_b200_decoder_layer* layer, float eps, 
 int rotor_b200_sample(const float* logits, int rows, int vocab, int mode, int top_k, float top_p,
                       float temperature, uint64_t seed, uint64_t counter, int64_t* out, void* stream);
 
+/* ---------------------------------------------------------------- beam search
+ * The reference samples; these two are the other way to generate: the best `count` continuations over a sequence's beams and
+ * the vocabulary, and the states that follow.
+ *  beam_select: a candidate is a token v after beam w of a group (the beams of one sequence), worth
+ *    scores[w] + logits[w][v] - log(sum_u exp(logits[w][u])); out are the `count` best of each group, best first, of equal
+ *    ones the lowest w, then the lowest v.  Values are compared in 64 bits and returned as float32.  `ended` (uint8
+ *    [groups][width] or NULL): a beam whose flag is set offers one candidate, (w, pad) with its score unchanged.  Logits that
+ *    are -inf or NaN offer nothing, nor does a row that holds +inf or a beam whose score is not finite; where fewer than
+ *    `count` candidates are left, the rest is filled with -inf and the lowest (w, v) that are not among them.
+ *    logits: `dtype` [groups][width][vocab], rows at group_stride and beam_stride elements; scores float32 [groups][width];
+ *    width <= 32, count <= 64 and <= width * vocab, width * vocab < 2^31.  out_scores float32, out_beams and out_tokens int64,
+ *    [groups][count].  workspace: rotor_b200_beam_select_workspace_bytes bytes, 16-byte aligned, contents of no matter.
+ *  reorder_states: row b * width + w of every state becomes what row b * width + beams[b][w] was, in place; rows whose beam is
+ *    their own, or no index of the group, stay.  `states` is a HOST array; width <= 32. */
+#define ROTOR_B200_F32 0
+#define ROTOR_B200_BF16 1
+#define ROTOR_B200_F16 2
+
+size_t rotor_b200_beam_select_workspace_bytes(int groups, int width, int vocab, int count);
+int rotor_b200_beam_select(const void* logits, int dtype, int64_t group_stride, int64_t beam_stride, const float* scores,
+                           const uint8_t* ended, int groups, int width, int vocab, int count, int64_t pad, float* out_scores,
+                           int64_t* out_beams, int64_t* out_tokens, void* workspace, size_t workspace_bytes, void* stream);
+
+/* Row r of a state holds `segments` pieces: segment_bytes bytes at data + r * row_stride + s * segment_stride. */
+typedef struct rotor_b200_state {
+    void* data;
+    size_t row_stride, segment_stride, segment_bytes;
+    int32_t segments;
+} rotor_b200_state;
+int rotor_b200_reorder_states(const rotor_b200_state* states, int n, const int64_t* beams, int groups, int width, void* stream);
+
+/* ---------------------------------------------------------------- 4-bit cache
+ * Keys and values of one layer in groups of 32 columns: m, the group's smallest value, and s = (largest - smallest) / 15, both
+ * float16, and per column the code of 0 .. 15 nearest to (x - m) / s (ties to even), which stands for m + s code.  s is the
+ * quotient rounded to float32, then to float16.  Magnitudes above 65504 are stored as 65504; NaN counts for neither bound and
+ * has code 0; a group of nothing else holds zeros.  The order of the codes inside a row is the library's own (read gives rows
+ * back in order).
+ *   codes [batch][kv_heads][max_seq][dim / 2]; steps and least values float16 [batch][kv_heads][max_seq][dim / 32]
+ * max_seq is a multiple of 16; dim 32, 64, 96, 128, 192 or 256; all six buffers 16-byte aligned and zero-filled before first use.
+ *
+ * Strides are HOST arrays of three (sequence, position, head), in elements; columns are neighbours.  `past`: positions each
+ * sequence holds already, or, with past_len (device int32 [batch], kept within 0 .. max_seq), past_len[b] of sequence b.
+ *  append: k, v `dtype` [batch][seq][kv_heads][dim] go to positions past .. past + seq - 1; those at max_seq and beyond are
+ *    not stored.
+ *  read: positions begin .. end - 1 of all sequences as k, v `dtype` [batch][kv_heads][end - begin][dim].
+ *  attend: q `dtype` [batch][seq][heads][dim] sits at positions past .. past + seq - 1 and sees cached positions j <= its own,
+ *    with window > 0 those with (own - j) < window.  Softmax of scale * q . k, whose denominator holds exp(sinks[head]) as well
+ *    (sinks float32 [heads] or NULL); query head h reads KV head h / (heads / kv_heads).  out: `dtype` [batch][seq][heads][dim],
+ *    16-byte aligned.  A query that sees no position gives zeros.  `longest`: with past_len, a bound of what a sequence holds
+ *    that the work is divided by (results do not depend on its being right); without, not read.  workspace:
+ *    rotor_b200_cache4_attend_workspace_bytes bytes with `longest` = past where past_len is NULL, 16-byte aligned, contents of no
+ *    matter. */
+typedef struct rotor_b200_cache4 {
+    int32_t batch, kv_heads, max_seq, dim;
+    uint8_t *k_codes, *v_codes;
+    void *k_step, *k_least, *v_step, *v_least;
+} rotor_b200_cache4;
+int rotor_b200_cache4_append(const rotor_b200_cache4* cache, const void* k, const void* v, int dtype, const int64_t* k_strides_host,
+                             const int64_t* v_strides_host, int seq, int past, const int32_t* past_len, void* stream);
+int rotor_b200_cache4_read(const rotor_b200_cache4* cache, int begin, int end, void* k, void* v, int dtype, void* stream);
+size_t rotor_b200_cache4_attend_workspace_bytes(const rotor_b200_cache4* cache, int heads, int seq, int longest, int window);
+int rotor_b200_cache4_attend(const rotor_b200_cache4* cache, const void* q, int dtype, const int64_t* q_strides_host, int heads, int seq,
+                             int past, const int32_t* past_len, int longest, float scale, int window, const float* sinks, void* out,
+                             void* workspace, size_t workspace_bytes, void* stream);
+
 /* ---------------------------------------------------------------- tensor parallel (new design)
  * The reference is single-device.  For models large enough to shard, BitLinear is split
  * Megatron-style over the GPUs of one box, one process per GPU: q/k/v, gate and up by output

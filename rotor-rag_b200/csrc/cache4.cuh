@@ -1,0 +1,111 @@
+// Keys and values of one layer in 4 bits.
+//
+// A row (one position of one KV head) is cut into groups of 32 columns.  Of a group are held m, its smallest value, and
+// s = (largest - smallest) / 15, both float16, and per column the code of 0 .. 15 nearest to (x - m) / s (the even one of two as
+// near); a code stands for m + s code.  128 columns take 80 bytes: 3.2 times less than bf16, 6.4 times less than float32.
+//
+// Codes lie in the order in which the attention's matrix instructions take them, so that a lane loads its part of a row in one piece
+// and no code is moved between lanes.  NG = dim / 32 groups:
+//   key row    four parts of NG words, one per lane of a quad: word j of part t holds columns 32 j + 8 t .. + 7, column 8 t + n in bits
+//              4 n .. 4 n + 3
+//   value row  eight parts of NG 16-bit words: word j of part g holds columns 32 j + 4 g .. + 3, column 4 g + n in bits 4 n .. 4 n + 3
+#pragma once
+#include <cuda_fp16.h>
+
+#include "decoder.cuh"
+
+namespace rb {
+
+constexpr int C4_GROUP = 32;
+constexpr int C4_POSITIONS = 16;    // max_seq is a multiple of this: a tile of the attention ends inside the cache
+constexpr float C4_MOST = 65504.f;  // magnitudes above the largest float16 are stored as that
+
+struct Cache4View {
+    uint8_t* codes[2];              // keys, values: [batch][kv_heads][max_seq][dim / 2]
+    __half *step[2], *least[2];     // [batch][kv_heads][max_seq][dim / 32]
+    int batch, kv_heads, max_seq, dim;
+};
+
+// x / d for x below 2^31, by a multiplication (a division by a number known at launch costs about twenty instructions).
+struct FastDiv {
+    uint32_t d, mul, shift;
+    __host__ explicit FastDiv(uint32_t n = 1) : d(n), shift(0) {
+        while ((1ull << shift) < n) ++shift;
+        mul = (uint32_t)((((1ull << shift) - n) << 32) / n + 1);
+    }
+    __device__ __forceinline__ uint32_t div(uint32_t x) const { return (__umulhi(x, mul) + x) >> shift; }
+};
+
+// Where sequence b of a call starts: a number for all, or one per sequence in device memory.
+struct Past {
+    const int* each;
+    int all;
+};
+__device__ __forceinline__ int past_of(const Past& p, int b, int max_seq) {
+    return p.each ? min(max(__ldcg(p.each + b), 0), max_seq) : p.all;
+}
+
+__device__ __forceinline__ float type_load(const float* p) { return *p; }
+__device__ __forceinline__ float type_load(const __nv_bfloat16* p) { return __bfloat162float(*p); }
+__device__ __forceinline__ float type_load(const __half* p) { return __half2float(*p); }
+
+// Eight neighbours as float32; `wide`: the address is a multiple of 16 bytes.
+__device__ __forceinline__ void load8(const float* p, bool wide, float (&x)[8]) {
+    if (wide) {
+        const float4 a = *reinterpret_cast<const float4*>(p), b = *reinterpret_cast<const float4*>(p + 4);
+        x[0] = a.x, x[1] = a.y, x[2] = a.z, x[3] = a.w, x[4] = b.x, x[5] = b.y, x[6] = b.z, x[7] = b.w;
+    } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) x[i] = p[i];
+    }
+}
+template <typename T2, typename T>
+__device__ __forceinline__ void load8_half(const T* p, bool wide, float (&x)[8]) {
+    if (wide) {
+        const uint4 v = *reinterpret_cast<const uint4*>(p);
+        const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const T2 h = *reinterpret_cast<const T2*>(&w[i]);
+            x[2 * i] = type_load(&h.x);
+            x[2 * i + 1] = type_load(&h.y);
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) x[i] = type_load(p + i);
+    }
+}
+__device__ __forceinline__ void load8(const __nv_bfloat16* p, bool wide, float (&x)[8]) { load8_half<__nv_bfloat162>(p, wide, x); }
+__device__ __forceinline__ void load8(const __half* p, bool wide, float (&x)[8]) { load8_half<__half2>(p, wide, x); }
+
+__device__ __forceinline__ void store8(float* p, const float (&x)[8]) {
+    *reinterpret_cast<float4*>(p) = make_float4(x[0], x[1], x[2], x[3]);
+    *reinterpret_cast<float4*>(p + 4) = make_float4(x[4], x[5], x[6], x[7]);
+}
+__device__ __forceinline__ void store8(__nv_bfloat16* p, const float (&x)[8]) {
+    const uint2 a = float4_to_bf16x4(make_float4(x[0], x[1], x[2], x[3])), b = float4_to_bf16x4(make_float4(x[4], x[5], x[6], x[7]));
+    *reinterpret_cast<uint4*>(p) = make_uint4(a.x, a.y, b.x, b.y);
+}
+__device__ __forceinline__ uint32_t pack_half(float lo, float hi) {
+    const __half2 h = __floats2half2_rn(lo, hi);
+    return *reinterpret_cast<const uint32_t*>(&h);
+}
+__device__ __forceinline__ void store8(__half* p, const float (&x)[8]) {
+    *reinterpret_cast<uint4*>(p) = make_uint4(pack_half(x[0], x[1]), pack_half(x[2], x[3]), pack_half(x[4], x[5]), pack_half(x[6], x[7]));
+}
+
+int cache4_view(const rotor_b200_cache4* c, Cache4View& v);  // checks the description
+
+// The positions [begin, begin + span) of every sequence and head as dense rows [batch][kv_heads][span][dim] of `dtype`; with `past`,
+// positions from past + seq on are zeros, and past goes to past_out as device words.
+struct Cache4Read {
+    Cache4View c;
+    void *k, *v;
+    int dtype, begin, span;
+    const Past* past;
+    int seq;
+    int* past_out;
+};
+int launch_cache4_read(const Cache4Read& r, cudaStream_t st);
+
+}  // namespace rb

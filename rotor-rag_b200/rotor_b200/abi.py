@@ -166,6 +166,33 @@ _SIGNATURES.update({
 })
 
 
+F32, BF16, F16 = 0, 1, 2
+
+
+class Cache4(C.Structure):
+    """rotor_b200_cache4"""
+    _fields_ = [("batch", C.c_int32), ("kv_heads", C.c_int32), ("max_seq", C.c_int32), ("dim", C.c_int32),
+                ("k_codes", _p), ("v_codes", _p), ("k_step", _p), ("k_least", _p), ("v_step", _p), ("v_least", _p)]
+
+
+class State(C.Structure):
+    """rotor_b200_state"""
+    _fields_ = [("data", _p), ("row_stride", _sz), ("segment_stride", _sz), ("segment_bytes", _sz), ("segments", C.c_int32)]
+
+
+_c4p, _i64, _sdp = C.POINTER(Cache4), C.c_int64, C.POINTER(C.c_int64)
+
+_SIGNATURES.update({
+    "rotor_b200_beam_select_workspace_bytes": (_sz, [_i, _i, _i, _i]),
+    "rotor_b200_beam_select": (_i, [_p, _i, _i64, _i64, _p, _p, _i, _i, _i, _i, _i64, _p, _p, _p, _p, _sz, _p]),
+    "rotor_b200_reorder_states": (_i, [C.POINTER(State), _i, _p, _i, _i, _p]),
+    "rotor_b200_cache4_append": (_i, [_c4p, _p, _p, _i, _sdp, _sdp, _i, _i, _p, _p]),
+    "rotor_b200_cache4_read": (_i, [_c4p, _i, _i, _p, _p, _i, _p]),
+    "rotor_b200_cache4_attend_workspace_bytes": (_sz, [_c4p, _i, _i, _i, _i]),
+    "rotor_b200_cache4_attend": (_i, [_c4p, _p, _i, _sdp, _i, _i, _i, _p, _i, _f, _i, _p, _p, _p, _sz, _p]),
+})
+
+
 def _declare(signatures):
     for name, (res, args) in signatures.items():
         if not os.path.exists(LIB_PATH) and not hasattr(lib, name):

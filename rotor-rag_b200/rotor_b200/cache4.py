@@ -1,0 +1,129 @@
+"""Keys and values of one layer in 4 bits, and attention over them.
+
+A row is held in groups of 32 columns: the group's smallest value and its step (largest - smallest) / 15, both float16, and a code of
+0 .. 15 per column.  128 columns take 80 bytes, 3.2 times less than in bfloat16.  Rows are quantised as they are written; the attention
+reads the codes themselves.
+"""
+from __future__ import annotations
+
+import ctypes as C
+
+from . import abi
+from .abi import RotorB200Error, check, lib
+from .ops import on_device, type_code
+
+GROUP = 32
+DIMS = (32, 64, 96, 128, 192, 256)
+
+
+class Cache4:
+    """``max_seq`` positions (rounded up to 16) of ``batch`` sequences: ``kv_heads`` heads of ``dim`` columns.
+
+    The caller keeps the sequences' lengths, as for the models' own caches: ``past`` is what they hold before a call, one number for
+    all or an int32 tensor [batch] on the device (a captured call reads it anew at every replay; values are kept within the cache).
+    Calls are ordered by the current stream."""
+
+    def __init__(self, batch: int, kv_heads: int, max_seq: int, dim: int):
+        if batch < 1 or kv_heads < 1 or max_seq < 1 or batch > 65535 or kv_heads > 65535 or max_seq > 1 << 26:
+            raise ValueError(f"a cache of {batch} sequences, {kv_heads} heads and {max_seq} positions")
+        if dim not in DIMS:
+            raise ValueError(f"heads of {dim} columns: {', '.join(map(str, DIMS))} are supported")
+        torch = abi.require_cuda()
+        self.batch, self.kv_heads, self.dim = batch, kv_heads, dim
+        self.max_seq = (max_seq + 15) // 16 * 16
+        make = lambda n, t: torch.zeros((batch, kv_heads, self.max_seq, n), dtype=t, device="cuda")
+        self.k_codes, self.v_codes = make(dim // 2, torch.uint8), make(dim // 2, torch.uint8)
+        self.k_step, self.k_least, self.v_step, self.v_least = (make(dim // GROUP, torch.float16) for _ in range(4))
+        self._c = abi.Cache4(batch, kv_heads, self.max_seq, dim, *(t.data_ptr() for t in self._tensors()))
+        self._ref = C.byref(self._c)
+
+    def _tensors(self):
+        return self.k_codes, self.v_codes, self.k_step, self.k_least, self.v_step, self.v_least
+
+    def states(self):
+        """For ``ops.reorder_states``: the tensors, each with the axis its positions run along."""
+        return [(t, 2) for t in self._tensors()]
+
+    def _past(self, past, seq):
+        """(number, address of the lengths or None), checked."""
+        if hasattr(past, "data_ptr"):
+            import torch
+            on_device("past", past, 1, torch.int32)
+            if past.shape[0] != self.batch or not past.is_contiguous():
+                raise ValueError(f"past of shape {tuple(past.shape)} for {self.batch} sequences")
+            if seq > self.max_seq:
+                raise ValueError(f"{seq} positions in a cache of {self.max_seq}")
+            return 0, past.data_ptr()
+        if past < 0 or past + seq > self.max_seq:
+            raise ValueError(f"positions {past} to {past + seq} in a cache of {self.max_seq}")
+        return past, None
+
+    def _rows(self, name, x, heads):
+        """Strides of rows [batch, seq, heads, dim], checked."""
+        on_device(name, x, 4)
+        b, s, h, d = x.shape
+        if b != self.batch or h != heads or d != self.dim:
+            raise ValueError(f"{name} of shape {(b, s, h, d)}, expected {(self.batch, 'positions', heads, self.dim)}")
+        sb, ss, sh, sd = x.stride()
+        if sd != 1:
+            raise ValueError(f"the columns of {name} have to lie side by side")
+        return (C.c_int64 * 3)(sb, ss, sh)
+
+    def append(self, k, v, past):
+        """Rows k and v [batch, seq, kv_heads, dim] (float32, bfloat16 or float16, any strides with columns side by side) are quantised
+        into the positions from ``past`` on; with a tensor of lengths, positions behind the end of the cache are left out."""
+        ks, vs = self._rows("k", k, self.kv_heads), self._rows("v", v, self.kv_heads)
+        if k.shape != v.shape or k.dtype is not v.dtype:
+            raise ValueError(f"k is {k.dtype} {tuple(k.shape)}, v is {v.dtype} {tuple(v.shape)}")
+        code, seq = type_code(k.dtype), k.shape[1]
+        number, lengths = self._past(past, seq)
+        if seq:
+            check(lib.rotor_b200_cache4_append(self._ref, k.data_ptr(), v.data_ptr(), code, ks, vs, seq, number, lengths, abi.stream()),
+                  "cache4_append")
+
+    def read(self, begin: int, end: int, dtype=None):
+        """What positions begin .. end - 1 stand for: keys and values [batch, kv_heads, end - begin, dim] (float32 unless told)."""
+        torch = abi.require_cuda()
+        dtype = dtype or torch.float32
+        if not 0 <= begin <= end <= self.max_seq:
+            raise ValueError(f"positions {begin} to {end} of a cache of {self.max_seq}")
+        code, shape = type_code(dtype), (self.batch, self.kv_heads, end - begin, self.dim)
+        k, v = torch.empty(shape, dtype=dtype, device="cuda"), torch.empty(shape, dtype=dtype, device="cuda")
+        if end > begin:
+            check(lib.rotor_b200_cache4_read(self._ref, begin, end, k.data_ptr(), v.data_ptr(), code, abi.stream()), "cache4_read")
+        return k, v
+
+    def attend(self, q, past, *, scale=None, window: int = 0, sinks=None, longest=None):
+        """Causal attention of queries [batch, seq, heads, dim] that sit at the positions from ``past`` on (their own keys and values
+        appended before) -> the same shape and type.
+
+        Query head h reads KV head h // (heads // kv_heads).  ``scale`` of the scores: 1 / sqrt(dim) unless given.  ``window`` > 0: a
+        query sees that many positions, its own included.  ``sinks`` float32 [heads]: exp(sink) joins the softmax's denominator.
+        ``longest``: with a tensor of lengths, the most that a sequence holds, by which the work is divided (the cache's size unless
+        given; a wrong bound costs time, not results).  A query that sees no position gives zeros."""
+        torch = abi.require_cuda()
+        heads = q.shape[2] if q.dim() == 4 else 0
+        strides = self._rows("q", q, heads)
+        if heads < 1 or heads % self.kv_heads:
+            raise ValueError(f"{heads} query heads cannot share {self.kv_heads} key/value heads evenly")
+        code, seq = type_code(q.dtype), q.shape[1]
+        number, lengths = self._past(past, seq)
+        if window < 0:
+            raise ValueError(f"a window of {window} positions")
+        if sinks is not None:
+            on_device("sinks", sinks, 1, torch.float32)
+            if sinks.shape[0] != heads or not sinks.is_contiguous():
+                raise ValueError("one sink per query head is needed")
+        out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+        if seq == 0:
+            return out
+        bound = number if lengths is None else self.max_seq if longest is None else min(max(int(longest), 0), self.max_seq)
+        need = lib.rotor_b200_cache4_attend_workspace_bytes(self._ref, heads, seq, bound, window)
+        if need == 0:
+            raise RotorB200Error(f"{seq} queries of {heads} heads are beyond the attention's sizes")
+        workspace = torch.empty(need, dtype=torch.uint8, device=q.device)
+        check(lib.rotor_b200_cache4_attend(self._ref, q.data_ptr(), code, strides, heads, seq, number, lengths, bound,
+                                           self.dim ** -0.5 if scale is None else float(scale), window,
+                                           None if sinks is None else sinks.data_ptr(), out.data_ptr(), workspace.data_ptr(), need,
+                                           abi.stream()), "cache4_attend")
+        return out
