@@ -1,11 +1,32 @@
 // The 4-bit cache is written and read back (layout: cache4.cuh).  Both directions move bytes: of a bf16 row of 128 columns 256 bytes
 // on the dense side and 80 in the cache.  A thread takes eight neighbouring columns, which are one word of a key row or two 16-bit words
-// of a value row, and four threads a group; threads run along rows, so that a warp's accesses are whole lines on both sides.
+// of a value tile, and four threads a group; threads run along rows.
 #include "cache4.cuh"
 
 namespace rb {
 
 constexpr int C4_THREADS = 256;
+
+// Where eight columns (c8 of a row) of a position lie: their word of the keys, or two 16-bit words of the values, `next` apart (parts g and
+// g + 1 of a tile), and their group's s and m.
+struct Place {
+    uint16_t* codes;
+    size_t group;
+    int next;
+    __device__ __forceinline__ Place(const Cache4View& c, int part, int b, uint32_t h, int pos, uint32_t c8) {
+        const int NG = c.dim / C4_GROUP, j = c8 >> 2, t = c8 & 3;
+        const size_t head = ((size_t)b * c.kv_heads + h) * c.max_seq;
+        if (part == 0) {
+            codes = reinterpret_cast<uint16_t*>(c.codes[0]) + (head + pos) * (NG * 8) + (t * NG + j) * 2;
+            group = (head + pos) * NG + j;
+            next = 1;
+        } else {
+            codes = reinterpret_cast<uint16_t*>(c.codes[1]) + (head + (pos & ~15)) * (NG * 8) + value_at(NG, j, 2 * t, pos & 15);
+            group = (head + (pos & ~3)) * NG + j * 4 + (pos & 3);
+            next = value_at(NG, j, 1, 0) - value_at(NG, j, 0, 0);
+        }
+    }
+};
 
 struct Cache4Store {
     Cache4View c;
@@ -32,7 +53,7 @@ __global__ void __launch_bounds__(C4_THREADS) cache4_store_kernel(const __grid_c
     pdl_wait();
     pdl_trigger();
     const uint32_t u = blockIdx.x * C4_THREADS + threadIdx.x;
-    const int b = blockIdx.y, part = blockIdx.z, NG = p.c.dim / C4_GROUP;
+    const int b = blockIdx.y, part = blockIdx.z;
     const bool on = u < p.units;
     const uint32_t row = p.per_row.div(on ? u : 0), c8 = (on ? u : 0) - row * p.per_row.d;
     const uint32_t i = p.heads.div(row), h = row - i * p.heads.d;
@@ -74,18 +95,16 @@ __global__ void __launch_bounds__(C4_THREADS) cache4_store_kernel(const __grid_c
     }
     const int pos = past_of(p.past, b, p.c.max_seq) + (int)i;
     if (!on || pos >= p.c.max_seq) return;
-    const size_t at = ((size_t)b * p.c.kv_heads + h) * p.c.max_seq + pos;
-    uint8_t* codes = p.c.codes[part] + at * (p.c.dim / 2);
-    const uint32_t j = c8 >> 2, t = c8 & 3;
+    const Place w(p.c, part, b, h, pos, c8);
     if (part == 0) {
-        *reinterpret_cast<uint32_t*>(codes + (t * NG + j) * 4) = word;
+        *reinterpret_cast<uint32_t*>(w.codes) = word;
     } else {
-        *reinterpret_cast<uint16_t*>(codes + (2 * t * NG + j) * 2) = (uint16_t)word;
-        *reinterpret_cast<uint16_t*>(codes + ((2 * t + 1) * NG + j) * 2) = (uint16_t)(word >> 16);
+        w.codes[0] = (uint16_t)word;
+        w.codes[w.next] = (uint16_t)(word >> 16);
     }
-    if (t == 0) {
-        p.c.step[part][at * NG + j] = sh;
-        p.c.least[part][at * NG + j] = mh;
+    if ((c8 & 3) == 0) {
+        p.c.step[part][w.group] = sh;
+        p.c.least[part][w.group] = mh;
     }
 }
 
@@ -93,9 +112,6 @@ struct Cache4Load {
     Cache4View c;
     void* dst[2];
     int begin, span;
-    int seq;         // > 0: positions from past + seq on are zeros
-    Past past;
-    int* past_out;
     uint32_t units;  // kv_heads * span * dim / 8
     FastDiv per_row, positions;
 };
@@ -105,27 +121,14 @@ __global__ void __launch_bounds__(C4_THREADS) cache4_load_kernel(const __grid_co
     pdl_wait();
     pdl_trigger();
     const uint32_t u = blockIdx.x * C4_THREADS + threadIdx.x;
-    const int b = blockIdx.y, part = blockIdx.z, NG = p.c.dim / C4_GROUP;
-    if (p.past_out && u == 0 && part == 0) p.past_out[b] = past_of(p.past, b, p.c.max_seq);
+    const int b = blockIdx.y, part = blockIdx.z;
     if (u >= p.units) return;
     const uint32_t row = p.per_row.div(u), c8 = u - row * p.per_row.d;
     const uint32_t h = p.positions.div(row), pos = p.begin + row - h * p.positions.d;
     float x[8];
-    const bool there = pos < (uint32_t)p.c.max_seq && (p.seq == 0 || (int)pos < past_of(p.past, b, p.c.max_seq) + p.seq);
-    const uint32_t j = c8 >> 2, t = c8 & 3;
-    uint32_t word = 0;
-    float s = 0.f, m = 0.f;
-    if (there) {
-        const size_t at = ((size_t)b * p.c.kv_heads + h) * p.c.max_seq + pos;
-        const uint8_t* codes = p.c.codes[part] + at * (p.c.dim / 2);
-        if (part == 0)
-            word = *reinterpret_cast<const uint32_t*>(codes + (t * NG + j) * 4);
-        else
-            word = *reinterpret_cast<const uint16_t*>(codes + (2 * t * NG + j) * 2) |
-                   (uint32_t) * reinterpret_cast<const uint16_t*>(codes + ((2 * t + 1) * NG + j) * 2) << 16;
-        s = __half2float(p.c.step[part][at * NG + j]);
-        m = __half2float(p.c.least[part][at * NG + j]);
-    }
+    const Place w(p.c, part, b, h, pos, c8);
+    const uint32_t word = part == 0 ? *reinterpret_cast<const uint32_t*>(w.codes) : w.codes[0] | (uint32_t)w.codes[w.next] << 16;
+    const float s = __half2float(p.c.step[part][w.group]), m = __half2float(p.c.least[part][w.group]);
 #pragma unroll
     for (int n = 0; n < 8; ++n) x[n] = fmaf((float)(word >> (4 * n) & 15u), s, m);
     store8(static_cast<T*>(p.dst[part]) + (((size_t)b * p.c.kv_heads + h) * p.span + (pos - p.begin)) * p.c.dim + c8 * 8, x);
@@ -163,9 +166,6 @@ int launch_cache4_read(const Cache4Read& r, cudaStream_t st) {
     p.dst[1] = r.v;
     p.begin = r.begin;
     p.span = r.span;
-    p.seq = r.past ? r.seq : 0;
-    p.past = r.past ? *r.past : Past{nullptr, 0};
-    p.past_out = r.past_out;
     p.units = (uint32_t)units;
     p.per_row = FastDiv(r.c.dim / 8);
     p.positions = FastDiv(r.span);

@@ -4,11 +4,13 @@
 // s = (largest - smallest) / 15, both float16, and per column the code of 0 .. 15 nearest to (x - m) / s (the even one of two as
 // near); a code stands for m + s code.  128 columns take 80 bytes: 3.2 times less than bf16, 6.4 times less than float32.
 //
-// Codes lie in the order in which the attention's matrix instructions take them, so that a lane loads its part of a row in one piece
-// and no code is moved between lanes.  NG = dim / 32 groups:
-//   key row    four parts of NG words, one per lane of a quad: word j of part t holds columns 32 j + 8 t .. + 7, column 8 t + n in bits
-//              4 n .. 4 n + 3
-//   value row  eight parts of NG 16-bit words: word j of part g holds columns 32 j + 4 g .. + 3, column 4 g + n in bits 4 n .. 4 n + 3
+// Everything lies in the order in which the attention's matrix instructions take it (m16n8k16, lane = 4 g + t), so that a lane loads its
+// part in whole pieces and nothing is moved between lanes.  NG = dim / 32 groups, j a group; inside a KV head's positions:
+//   key codes    [position][t][j] words: columns 32 j + 8 t .. + 7, column 8 t + n in bits 4 n .. 4 n + 3
+//   key s, m     [position][j]
+//   value codes  tiles of 16 positions; [j][lane][position % 4] 16-bit words, t = position % 16 / 4: columns 32 j + 4 g .. + 3, column
+//                4 g + n in bits 4 n .. 4 n + 3; two groups' words of a lane are neighbours (value_at)
+//   value s, m   [position / 4][j][position % 4]
 #pragma once
 #include <cuda_fp16.h>
 
@@ -20,9 +22,15 @@ constexpr int C4_GROUP = 32;
 constexpr int C4_POSITIONS = 16;    // max_seq is a multiple of this: a tile of the attention ends inside the cache
 constexpr float C4_MOST = 65504.f;  // magnitudes above the largest float16 are stored as that
 
+// Place of group j's word of position % 16 = r, part g, in a tile of value codes, in 16-bit words.
+__host__ __device__ __forceinline__ int value_at(int NG, int j, int g, int r) {
+    const int lane = 4 * g + (r >> 2);
+    return (j < NG / 2 * 2 ? j / 2 * 256 + lane * 8 + j % 2 * 4 : NG / 2 * 256 + lane * 4) + (r & 3);
+}
+
 struct Cache4View {
     uint8_t* codes[2];              // keys, values: [batch][kv_heads][max_seq][dim / 2]
-    __half *step[2], *least[2];     // [batch][kv_heads][max_seq][dim / 32]
+    __half *step[2], *least[2];     // s and m: [batch][kv_heads][max_seq][dim / 32]
     int batch, kv_heads, max_seq, dim;
 };
 
@@ -96,15 +104,12 @@ __device__ __forceinline__ void store8(__half* p, const float (&x)[8]) {
 
 int cache4_view(const rotor_b200_cache4* c, Cache4View& v);  // checks the description
 
-// The positions [begin, begin + span) of every sequence and head as dense rows [batch][kv_heads][span][dim] of `dtype`; with `past`,
-// positions from past + seq on are zeros, and past goes to past_out as device words.
+
+// The positions [begin, begin + span) of every sequence and head as dense rows [batch][kv_heads][span][dim] of `dtype`.
 struct Cache4Read {
     Cache4View c;
     void *k, *v;
     int dtype, begin, span;
-    const Past* past;
-    int seq;
-    int* past_out;
 };
 int launch_cache4_read(const Cache4Read& r, cudaStream_t st);
 

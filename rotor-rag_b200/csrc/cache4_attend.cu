@@ -7,15 +7,18 @@
 // Codes are multiplied as they are: a code in the low bits of a float16 is the (subnormal) number code 2^-24, exactly, and one AND makes
 // two of them; in the next four bits it is code 2^-20.  No code is converted, and nothing of a cached row is rounded.  The queries of
 // 16-bit types are exact in the other operand (a row is scaled by a power of two into float16's range; columns whose codes lie four bits
-// higher by another 1/16), float32 queries are split into two terms (2^-22 of the value).  The weights p_j s_jg are rounded to float16
-// (2^-12 of the weight; in float32 calls two terms again).  Scores, maxima, sums and outputs are float32.
-//
-// The shift of the softmax is the running maximum of score + log2(largest s_jg of the row), not of the score: p s is then at most 1 times
-// the shift's slack whatever the values' size is, and stays in float16's range.
+// higher by another 1/16), float32 queries are split into two terms (2^-22 of the value).  The weights p_j are rounded to float16 and so
+// are their products with s_jg (2^-12 each; the sum of weights takes them as rounded), in float32 calls both are two terms (2^-22).
+// Scores, maxima, sums and outputs are float32.  Matrix instructions cut their sums off instead of rounding them, which shows after many
+// of them in a row: float32 calls begin every tile's sums at zero and add them up outside.
 //
 // A warp takes tiles of 16 positions and keeps eight (R = 1) or sixteen (R = 2) query rows of one KV head (row = token x query head of the
-// group): scores by m16n8k16 with queries as rows and positions as columns, whose result is the operand that the second product
-// (columns of V as rows, queries as columns) takes, without an exchange between lanes.
+// group).  Both products have the codes as their 16-row operand: S = K Q^T (positions x queries) and O^T = V^T P (columns x queries);
+// two 8 x 8 transposes (movmatrix) turn the weights from the one's result into the other's operand.  One more instruction per tile sums
+// p m over the groups and, in a row of ones, p itself.
+//
+// Tiles travel by cp.async into a ring of the warp's own (no barrier, and the loads in flight do not depend on what the registers hold):
+// a tile of 128 columns is 2560 bytes, five copies a lane.
 #include <cmath>
 
 #include "cache4.cuh"
@@ -23,8 +26,10 @@
 namespace rb {
 
 constexpr int A4_WARPS = 8, A4_THREADS = 32 * A4_WARPS;
-constexpr float A4_SLACK = 8.f;   // a new maximum below the old one plus this (in powers of two) leaves the shift where it is
-constexpr float A4_LIFT = 7.f;    // weights are at most 2^(A4_SLACK + A4_LIFT), and use float16's range down to 2^-24
+constexpr float A4_SLACK = 7.f;   // a new maximum below the old one plus this (in powers of two) leaves the shift where it is
+constexpr float A4_LIFT = 7.f;    // weights are at most 2^(lift + slack): p s below 2^15 for s below 2, and a smaller lift for larger s
+constexpr float A4_LOW = -1e30f;  // a shift that any score is above
+constexpr int A4_CLUSTER = 8;     // most splits that are joined inside a cluster
 
 struct Attend4 {
     Cache4View c;
@@ -53,370 +58,103 @@ __device__ __forceinline__ void a4_mma(float (&d)[4], uint32_t a0, uint32_t a1, 
 
 __device__ __forceinline__ float2 half2_of(uint32_t v) { return __half22float2(*reinterpret_cast<const __half2*>(&v)); }
 
-// N bytes at an address that is a multiple of the largest power of two that divides N (up to 16), as words.
+// N bytes of shared memory at an address that is a multiple of the largest power of two that divides N (up to 16), as words.
 template <int N>
 struct Bytes {
     static constexpr int W = (N + 3) / 4;
     uint32_t w[W];
-    __device__ __forceinline__ void load(const void* p) {
+    __device__ __forceinline__ void load(const unsigned char* p) {
         if constexpr (N % 16 == 0) {
 #pragma unroll
             for (int i = 0; i < N / 16; ++i) {
-                const uint4 v = __ldcg(reinterpret_cast<const uint4*>(p) + i);
+                const uint4 v = reinterpret_cast<const uint4*>(p)[i];
                 w[4 * i] = v.x, w[4 * i + 1] = v.y, w[4 * i + 2] = v.z, w[4 * i + 3] = v.w;
             }
         } else if constexpr (N % 8 == 0) {
 #pragma unroll
             for (int i = 0; i < N / 8; ++i) {
-                const uint2 v = __ldcg(reinterpret_cast<const uint2*>(p) + i);
+                const uint2 v = reinterpret_cast<const uint2*>(p)[i];
                 w[2 * i] = v.x, w[2 * i + 1] = v.y;
             }
         } else if constexpr (N % 4 == 0) {
 #pragma unroll
-            for (int i = 0; i < N / 4; ++i) w[i] = __ldcg(reinterpret_cast<const uint32_t*>(p) + i);
+            for (int i = 0; i < N / 4; ++i) w[i] = reinterpret_cast<const uint32_t*>(p)[i];
         } else {
             static_assert(N % 2 == 0, "16-bit pieces");
 #pragma unroll
             for (int i = 0; i < W; ++i) w[i] = 0;
 #pragma unroll
-            for (int i = 0; i < N / 2; ++i) w[i / 2] |= (uint32_t)__ldcg(reinterpret_cast<const unsigned short*>(p) + i) << (16 * (i & 1));
+            for (int i = 0; i < N / 2; ++i) w[i / 2] |= (uint32_t)reinterpret_cast<const unsigned short*>(p)[i] << (16 * (i & 1));
         }
     }
-    // the 16-bit piece i
-    __device__ __forceinline__ uint32_t piece(int i) const { return w[i >> 1] >> (16 * (i & 1)) & 0xffffu; }
-};
-
-// What a lane (g = lane / 4, t = lane % 4) needs of a tile: column c of the scores' part u is position 4 (c / 2) + 2 u + c % 2, so that a
-// lane's four scores of a row are those of positions 4 t .. 4 t + 3, in order.
-template <int NG>
-struct Tile4 {
-    Bytes<4 * NG> k[2];                 // part t of the key rows 4 (g / 2) + 2 u + g % 2
-    Bytes<2 * NG> v[4];                 // part g of the value rows 4 t + i
-    Bytes<8 * NG> ks, vs, vm;           // rows 4 t .. 4 t + 3
-    uint32_t km[2];                     // two groups' m of the key rows of k[]
-    __device__ __forceinline__ void load(const Cache4View& c, size_t row0, int g, int t) {
-#pragma unroll
-        for (int u = 0; u < 2; ++u) {
-            const size_t r = row0 + 4 * (g >> 1) + 2 * u + (g & 1);
-            k[u].load(c.codes[0] + r * (16 * NG) + t * 4 * NG);
-            const __half* m = c.least[0] + r * NG;
-            // the matrix instruction that multiplies the m takes a pair of groups per lane (see the queries' sums)
-            const int pair = NG > 4 ? 2 * t : 2 * (t & 1);
-            const unsigned short* mu = reinterpret_cast<const unsigned short*>(m) + pair;
-            if constexpr (NG % 2 == 0)
-                km[u] = pair < NG ? __ldcg(reinterpret_cast<const uint32_t*>(mu)) : 0u;
-            else
-                km[u] = (pair < NG ? __ldcg(mu) : 0u) | (uint32_t)(pair + 1 < NG ? __ldcg(mu + 1) : 0u) << 16;
-        }
-#pragma unroll
-        for (int i = 0; i < 4; ++i) v[i].load(c.codes[1] + (row0 + 4 * t + i) * (16 * NG) + g * 2 * NG);
-        ks.load(c.step[0] + (row0 + 4 * t) * NG);
-        vs.load(c.step[1] + (row0 + 4 * t) * NG);
-        vm.load(c.least[1] + (row0 + 4 * t) * NG);
-    }
-    static __device__ __forceinline__ float half_at(const Bytes<8 * NG>& b, int i) {
-        const float2 f = half2_of(b.w[i >> 1]);
+    __device__ __forceinline__ float half_at(int i) const {
+        const float2 f = half2_of(w[i >> 1]);
         return i & 1 ? f.y : f.x;
     }
 };
 
-template <int NG, int R>
-struct Attend4Smem {
-    static constexpr int D = 32 * NG, Q = 8 * R, OS = D + 4;  // (a row of sums is four floats longer: lanes of a quad on other banks)
-    float sums[A4_WARPS][Q][OS];
-    float shift[A4_WARPS][Q], mass[A4_WARPS][Q];
-};
-template <int NG, int R, int TERMS>
-struct Attend4Query {
-    uint4 frag[NG][TERMS][R][32];  // the queries as operands: per lane a0, a2 (or a1, a3) of a group's two steps of 16 columns
-    float top[NG][8 * R], sum[NG][8 * R];
-};
-
-template <int NG, int R, int TERMS>
-__global__ void __launch_bounds__(A4_THREADS) attend4_kernel(const __grid_constant__ Attend4 p) {
-    constexpr int D = 32 * NG, Q = 8 * R;
-    using Smem = Attend4Smem<NG, R>;
-    using Query = Attend4Query<NG, R, TERMS>;
-    extern __shared__ __align__(16) unsigned char a4_raw[];
-    Query& sq = *reinterpret_cast<Query*>(a4_raw);
-    Smem& sm = *reinterpret_cast<Smem*>(a4_raw);  // (takes the queries' place at the end)
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
-    const int blocks = (p.rows + Q - 1) / Q;
-    const int hk = blockIdx.x / blocks, r0 = (blockIdx.x - hk * blocks) * Q, b = blockIdx.z, split = blockIdx.y;
-    pdl_wait();
-    pdl_trigger();
-
-    const int past = past_of(p.past, b, p.c.max_seq), last_row = min(r0 + Q, p.rows) - 1;
-    const int lo_block = first_visible(past + r0 / p.group, 0, p.window);
-    const int hi_block = min(past + last_row / p.group, p.c.max_seq - 1);
-    const int tile0 = lo_block / 16, tiles = hi_block / 16 + 1 - tile0;
-    const int per = (max(tiles, 0) + p.splits - 1) / p.splits;
-    const int first = tile0 + split * per, end = min(first + per, tile0 + tiles);
-
-    // ---- queries: warp j makes the operands of group j
-    float qv[R][8], inv_fs[R];
-    int lo[R], hi[R];
-#pragma unroll
-    for (int h = 0; h < R; ++h) {
-        const int row = r0 + g + 8 * h, token = min(row, last_row) / p.group, head = hk * p.group + min(row, last_row) - token * p.group;
-        lo[h] = first_visible(past + token, 0, p.window);
-        hi[h] = row <= last_row ? min(past + token, p.c.max_seq - 1) : -1;
-        float top = 0.f;
-        if (warp < NG) {
-            const size_t at = (size_t)b * p.qb + (size_t)token * p.qs + (size_t)head * p.qh + 32 * warp + 8 * t;
-            if (p.dtype == ROTOR_B200_F32)
-                load8(static_cast<const float*>(p.q) + at, p.wide, qv[h]);
-            else if (p.dtype == ROTOR_B200_BF16)
-                load8(static_cast<const __nv_bfloat16*>(p.q) + at, p.wide, qv[h]);
-            else
-                load8(static_cast<const __half*>(p.q) + at, p.wide, qv[h]);
-            float sum = 0.f;
-#pragma unroll
-            for (int n = 0; n < 8; ++n) {
-                top = fmaxf(top, fabsf(qv[h][n]));
-                sum += qv[h][n];
-            }
-#pragma unroll
-            for (int o = 1; o < 4; o <<= 1) {
-                top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-                sum += __shfl_xor_sync(0xffffffffu, sum, o);
-            }
-            if (t == 0) {
-                sq.top[warp][g + 8 * h] = top;
-                sq.sum[warp][g + 8 * h] = sum;
-            }
-        }
-    }
-    __syncthreads();
-    uint32_t sum_hi[R], sum_lo[R];  // operands: sums of the queries over the groups' columns, as two terms
-#pragma unroll
-    for (int h = 0; h < R; ++h) {
-        float top = 0.f;
-#pragma unroll
-        for (int j = 0; j < NG; ++j) top = fmaxf(top, sq.top[j][g + 8 * h]);
-        // a power of two that takes the row's largest value to 2^14 .. 2^15 (none for rows of zeros, infinities and NaN)
-        const int e = (__float_as_int(top) >> 23) - 127;
-        const bool scaled = top > 0.f && e < 128;
-        const int up = scaled ? min(14 - e, 100) : 0;
-        const float fs = __int_as_float((127 + up) << 23);
-        inv_fs[h] = __int_as_float((127 - up) << 23);
-        if (warp < NG) {
-            float x[8];
-#pragma unroll
-            for (int n = 0; n < 8; ++n) x[n] = qv[h][n] * (n & 1 ? fs * 0.0625f : fs);
-#pragma unroll
-            for (int term = 0; term < TERMS; ++term) {
-                const uint4 f = make_uint4(pack_half(x[0], x[4]), pack_half(x[2], x[6]), pack_half(x[1], x[5]), pack_half(x[3], x[7]));
-                sq.frag[warp][term][h][lane] = f;
-                if (TERMS > 1) {
-                    const float2 a = half2_of(f.x), c = half2_of(f.y), d = half2_of(f.z), w = half2_of(f.w);
-                    x[0] -= a.x, x[4] -= a.y, x[2] -= c.x, x[6] -= c.y, x[1] -= d.x, x[5] -= d.y, x[3] -= w.x, x[7] -= w.y;
-                }
-            }
-        }
-        const int pair = NG > 4 ? 2 * t : 2 * (t & 1);
-        const float f6 = fs * 0.015625f;  // (the sum of 32 columns is up to 2^20 and has to fit as well)
-        const float s0 = pair < NG ? sq.sum[pair][g + 8 * h] * f6 : 0.f, s1 = pair + 1 < NG ? sq.sum[pair + 1][g + 8 * h] * f6 : 0.f;
-        const uint32_t big = pack_half(s0, s1);
-        const float2 bf = half2_of(big);
-        const uint32_t rest = pack_half(s0 - bf.x, s1 - bf.y);
-        if (NG > 4) {
-            sum_hi[h] = big;
-            sum_lo[h] = rest;
-        } else {  // up to four groups: lanes 0 and 1 of a quad hold the first terms, 2 and 3 the second ones
-            sum_hi[h] = t < 2 ? big : rest;
-            sum_lo[h] = 0u;
-        }
-    }
-    __syncthreads();
-
-    float shift[R], mass[R], low_sum[R][NG];
-    float o[R][2 * NG][4];
-#pragma unroll
-    for (int h = 0; h < R; ++h) {
-        shift[h] = -INFINITY;
-        mass[h] = 0.f;
-#pragma unroll
-        for (int j = 0; j < NG; ++j) low_sum[h][j] = 0.f;
-#pragma unroll
-        for (int i = 0; i < 2 * NG; ++i)
-#pragma unroll
-            for (int n = 0; n < 4; ++n) o[h][i][n] = 0.f;
-    }
-    const size_t head_row = ((size_t)b * p.c.kv_heads + hk) * p.c.max_seq;
-    for (int tile = first + warp; tile < end; tile += A4_WARPS) {
-        Tile4<NG> x;
-        x.load(p.c, head_row + (size_t)tile * 16, g, t);
-
-        // ---- scores of 8 R rows x 16 positions: lane's four positions of row g (and g + 8)
-        float sc[R][4];
-#pragma unroll
-        for (int h = 0; h < R; ++h)
-#pragma unroll
-            for (int i = 0; i < 4; ++i) sc[h][i] = 0.f;
-#pragma unroll
-        for (int j = 0; j < NG; ++j) {
-            float acc[2][4] = {};
-            const uint32_t w0 = x.k[0].w[j], w1 = x.k[1].w[j];
-#pragma unroll
-            for (int term = 0; term < TERMS; ++term) {
-                const uint4 fa = sq.frag[j][term][0][lane];
-                const uint4 fb = R > 1 ? sq.frag[j][term][R - 1][lane] : make_uint4(0u, 0u, 0u, 0u);
-                a4_mma(acc[0], fa.x, fb.x, fa.y, fb.y, w0 & 0x000f000fu, w0 >> 8 & 0x000f000fu);
-                a4_mma(acc[1], fa.x, fb.x, fa.y, fb.y, w1 & 0x000f000fu, w1 >> 8 & 0x000f000fu);
-                a4_mma(acc[0], fa.z, fb.z, fa.w, fb.w, w0 & 0x00f000f0u, w0 >> 8 & 0x00f000f0u);
-                a4_mma(acc[1], fa.z, fb.z, fa.w, fb.w, w1 & 0x00f000f0u, w1 >> 8 & 0x00f000f0u);
-            }
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const float s = Tile4<NG>::half_at(x.ks, i * NG + j);
-#pragma unroll
-                for (int h = 0; h < R; ++h) sc[h][i] = fmaf(s, acc[i >> 1][2 * h + (i & 1)], sc[h][i]);
-            }
-        }
-        float low[2][4] = {};
-#pragma unroll
-        for (int u = 0; u < 2; ++u)
-            a4_mma(low[u], sum_hi[0], R > 1 ? sum_hi[R - 1] : 0u, NG > 4 ? sum_lo[0] : 0u, NG > 4 && R > 1 ? sum_lo[R - 1] : 0u, x.km[u],
-                   NG > 4 ? x.km[u] : 0u);
-
-        // ---- largest step of each position's value row, as a power of two
-        float ls[4];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            float m = 5.9604645e-8f;  // the smallest float16 above zero
-#pragma unroll
-            for (int j = 0; j < NG; ++j) m = fmaxf(m, Tile4<NG>::half_at(x.vs, i * NG + j));
-            ls[i] = __log2f(m);
-        }
-        const int pos = tile * 16 + 4 * t;
-        float tmax[R];
-        bool higher = false;
-#pragma unroll
-        for (int h = 0; h < R; ++h) {
-            const float f = p.scale2 * inv_fs[h];
-            tmax[h] = -INFINITY;
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                sc[h][i] = (sc[h][i] * 16777216.f + low[i >> 1][2 * h + (i & 1)] * 64.f) * f;
-                if (pos + i < lo[h] || pos + i > hi[h]) sc[h][i] = -INFINITY;
-                tmax[h] = fmaxf(tmax[h], sc[h][i] + ls[i]);
-            }
-            higher |= tmax[h] - A4_LIFT > shift[h] + A4_SLACK;
-        }
-        if (__any_sync(0xffffffffu, higher)) {
-#pragma unroll
-            for (int h = 0; h < R; ++h) {
-                float m = tmax[h];
-                m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 1));
-                m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 2));
-                m = fmaxf(shift[h], m - A4_LIFT);
-                const float alpha = m == shift[h] ? 1.f : a4_exp2(shift[h] - m);
-                shift[h] = m;
-                mass[h] *= alpha;
-#pragma unroll
-                for (int j = 0; j < NG; ++j) low_sum[h][j] *= alpha;
-                // the sums' columns are query rows 2 t and 2 t + 1
-                const float a0 = __shfl_sync(0xffffffffu, alpha, 8 * t), a1 = __shfl_sync(0xffffffffu, alpha, 8 * t + 4);
-#pragma unroll
-                for (int i = 0; i < 2 * NG; ++i) {
-                    o[h][i][0] *= a0;
-                    o[h][i][1] *= a1;
-                    o[h][i][2] *= a0;
-                    o[h][i][3] *= a1;
-                }
-            }
-        }
-#pragma unroll
-        for (int h = 0; h < R; ++h) {
-            const float m = shift[h] == -INFINITY ? 0.f : shift[h];
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                sc[h][i] = a4_exp2(sc[h][i] - m);
-                mass[h] += sc[h][i];
-            }
-        }
-
-        // ---- sums over the positions
-#pragma unroll
-        for (int j = 0; j < NG; ++j) {
-            const uint32_t y01 = x.v[0].piece(j) | x.v[1].piece(j) << 16, y23 = x.v[2].piece(j) | x.v[3].piece(j) << 16;
-            float s[4], m[4];
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                s[i] = Tile4<NG>::half_at(x.vs, i * NG + j);
-                m[i] = Tile4<NG>::half_at(x.vm, i * NG + j);
-            }
-#pragma unroll
-            for (int h = 0; h < R; ++h) {
-                float w[4];
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    w[i] = sc[h][i] * s[i];
-                    low_sum[h][j] = fmaf(sc[h][i], m[i], low_sum[h][j]);
-                }
-#pragma unroll
-                for (int term = 0; term < TERMS; ++term) {
-                    const uint32_t b0 = pack_half(w[0], w[1]), b1 = pack_half(w[2], w[3]);
-                    a4_mma(o[h][2 * j], y01 & 0x000f000fu, y01 & 0x00f000f0u, y23 & 0x000f000fu, y23 & 0x00f000f0u, b0, b1);
-                    a4_mma(o[h][2 * j + 1], y01 >> 8 & 0x000f000fu, y01 >> 8 & 0x00f000f0u, y23 >> 8 & 0x000f000fu, y23 >> 8 & 0x00f000f0u, b0,
-                           b1);
-                    if (TERMS > 1) {
-                        const float2 f0 = half2_of(b0), f1 = half2_of(b1);
-                        w[0] -= f0.x, w[1] -= f0.y, w[2] -= f1.x, w[3] -= f1.y;
-                    }
-                }
-            }
-        }
-    }
-
-    // ---- the warps' sums are joined in shared memory
-    __syncthreads();  // (the last query operand has been read)
-#pragma unroll
-    for (int h = 0; h < R; ++h) {
-#pragma unroll
-        for (int n = 1; n < 4; n <<= 1) {
-            mass[h] += __shfl_xor_sync(0xffffffffu, mass[h], n);
-#pragma unroll
-            for (int j = 0; j < NG; ++j) low_sum[h][j] += __shfl_xor_sync(0xffffffffu, low_sum[h][j], n);
-        }
-        if (t == 0) {
-            sm.shift[warp][8 * h + g] = shift[h];
-            sm.mass[warp][8 * h + g] = mass[h];
-        }
-#pragma unroll
-        for (int j = 0; j < NG; ++j) {
-            // columns 32 j + 4 g .. + 3 of query rows 2 t and 2 t + 1; sums of codes four bits higher are 16 times too large
-            const float l0 = __shfl_sync(0xffffffffu, low_sum[h][j], 8 * t), l1 = __shfl_sync(0xffffffffu, low_sum[h][j], 8 * t + 4);
-            constexpr float c0 = 16777216.f, c1 = 1048576.f;
-            const float(&a)[4] = o[h][2 * j], (&c)[4] = o[h][2 * j + 1];
-            *reinterpret_cast<float4*>(&sm.sums[warp][8 * h + 2 * t][32 * j + 4 * g]) =
-                make_float4(fmaf(a[0], c0, l0), fmaf(a[2], c1, l0), fmaf(c[0], c0, l0), fmaf(c[2], c1, l0));
-            *reinterpret_cast<float4*>(&sm.sums[warp][8 * h + 2 * t + 1][32 * j + 4 * g]) =
-                make_float4(fmaf(a[1], c0, l1), fmaf(a[3], c1, l1), fmaf(c[1], c0, l1), fmaf(c[3], c1, l1));
-        }
-    }
-    __syncthreads();
-    for (int idx = threadIdx.x; idx < Q * (D / 4); idx += A4_THREADS) {
-        const int r = idx / (D / 4), c4 = idx - r * (D / 4), row = r0 + r;
-        if (row >= p.rows) break;
-        float top = -INFINITY, total = 0.f;
-#pragma unroll
-        for (int w = 0; w < A4_WARPS; ++w) top = fmaxf(top, sm.shift[w][r]);
-        float4 y = make_float4(0.f, 0.f, 0.f, 0.f);
-        const float ref = top == -INFINITY ? 0.f : top;  // (a warp without a visible position: its zeros times zero; NaN stays)
-#pragma unroll
-        for (int w = 0; w < A4_WARPS; ++w) {
-            const float f = a4_exp2(sm.shift[w][r] - ref);
-            const float4 v = *reinterpret_cast<const float4*>(&sm.sums[w][r][4 * c4]);
-            total = fmaf(f, sm.mass[w][r], total);
-            y.x = fmaf(f, v.x, y.x), y.y = fmaf(f, v.y, y.y), y.z = fmaf(f, v.z, y.z), y.w = fmaf(f, v.w, y.w);
-        }
-        float* part = p.part + (((size_t)(b * p.c.kv_heads + hk) * p.rows + row) * p.splits + split) * (D + 4);
-        *reinterpret_cast<float4*>(part + 4 * c4) = y;
-        if (c4 == 0) *reinterpret_cast<float2*>(part + D) = make_float2(top, total);
-    }
+__device__ __forceinline__ uint32_t turned(uint32_t v) {  // the 8 x 8 matrix of 16-bit numbers, transposed
+    uint32_t r;
+    asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));
+    return r;
 }
+__device__ __forceinline__ __half2 as_half2(uint32_t v) { return *reinterpret_cast<const __half2*>(&v); }
+__device__ __forceinline__ uint32_t as_word(__half2 v) { return *reinterpret_cast<const uint32_t*>(&v); }
+
+__device__ __forceinline__ void copy16(uint32_t dst, const void* src) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+}
+__device__ __forceinline__ void copy_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void copy_wait() {
+    asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
+
+// A tile in shared memory: key codes, value codes, then s and m of the keys and of the values.
+template <int NG>
+struct Tile4 {
+    static constexpr int V = 256 * NG, KS = 512 * NG, KM = 544 * NG, VS = 576 * NG, VM = 608 * NG, BYTES = 640 * NG;
+    // 16-byte pieces: 16 NG of each kind of codes, 8 NG of s and m; pieces lane + 32 r of a lane's rounds
+    static constexpr int CODE_ROUNDS = (NG + 1) / 2, REST_ROUNDS = (NG + 3) / 4;
+    const unsigned char *k, *v, *rest[REST_ROUNDS];  // where this lane's pieces of tile 0 of the head are
+    __device__ __forceinline__ Tile4(const Cache4View& c, size_t head_row, int lane) {
+        k = c.codes[0] + head_row * (16 * NG) + lane * 16;
+        v = c.codes[1] + head_row * (16 * NG) + lane * 16;
+        const __half* kinds[4] = {c.step[0], c.least[0], c.step[1], c.least[1]};
+#pragma unroll
+        for (int r = 0; r < REST_ROUNDS; ++r) {
+            const int piece = lane + 32 * r, kind = min(piece / (2 * NG), 3);
+            const __half* base = kind == 0 ? kinds[0] : kind == 1 ? kinds[1] : kind == 2 ? kinds[2] : kinds[3];
+            rest[r] = reinterpret_cast<const unsigned char*>(base + head_row * NG) + (piece - kind * 2 * NG) * 16;
+        }
+    }
+    __device__ __forceinline__ void fetch(int tile, uint32_t dst, int lane) const {
+#pragma unroll
+        for (int r = 0; r < CODE_ROUNDS; ++r) {
+            if (NG % 2 == 0 || lane + 32 * r < 16 * NG) {
+                copy16(dst + (lane + 32 * r) * 16, k + (size_t)tile * V + 512 * r);
+                copy16(dst + V + (lane + 32 * r) * 16, v + (size_t)tile * V + 512 * r);
+            }
+        }
+#pragma unroll
+        for (int r = 0; r < REST_ROUNDS; ++r)
+            if (NG % 4 == 0 || lane + 32 * r < 8 * NG) copy16(dst + KS + (lane + 32 * r) * 16, rest[r] + (size_t)tile * (32 * NG));
+    }
+};
+
+template <int NG, int R, int TERMS>
+struct A4Cfg {
+    static constexpr int D = 32 * NG, Q = 8 * R;
+    static constexpr int STAGES = NG >= 6 ? 2 : 3;
+    static constexpr int OS = D + 4;             // floats between a row's sums and the next: lanes of a quad on other banks
+    static constexpr bool KEEP = NG * R * TERMS <= 4;  // the queries' operands stay in registers
+    // queries as operands: per lane two pairs of a group's two steps of 16 columns; largest values and sums of the groups
+    static constexpr int FRAG = 0, TOPS = FRAG + NG * TERMS * R * 512, SUMS = TOPS + NG * Q * 4, RING = SUMS + NG * Q * 4;
+    static constexpr int RING_BYTES = A4_WARPS * STAGES * Tile4<NG>::BYTES;
+    // at the end, over the ring: sums of the warps' rows, shifts, masses; then the CTA's rows for the cluster
+    static constexpr int O = RING, SHIFT = O + A4_WARPS * Q * OS * 4, MASS = SHIFT + A4_WARPS * Q * 4, ROWS = MASS + A4_WARPS * Q * 4;
+    static constexpr int END = ROWS + Q * OS * 4, SMEM = END > RING + RING_BYTES ? END : RING + RING_BYTES;
+};
 
 __device__ __forceinline__ void store4(void* out, int dtype, size_t at, float4 y) {
     if (dtype == ROTOR_B200_F32) {
@@ -428,30 +166,412 @@ __device__ __forceinline__ void store4(void* out, int dtype, size_t at, float4 y
     }
 }
 
-// Joins the splits of a query row: a warp per row and 128 columns.
+// Four columns of a query row from the sums y, their mass and shift.  A row that sees no position gives zeros.
+__device__ __forceinline__ void finish4(const Attend4& p, int b, int hk, int row, int col, float4 y, float mass, float shift) {
+    const int token = row / p.group, head = hk * p.group + row - token * p.group;
+    if (p.sinks) {
+        const float sink = __ldg(p.sinks + head) * 1.4426950408889634f, top = fmaxf(shift, sink), mine = a4_exp2(shift - top);
+        mass = fmaf(mass, mine, a4_exp2(sink - top));
+        y.x *= mine, y.y *= mine, y.z *= mine, y.w *= mine;
+    }
+    const float inv = mass == 0.f ? 0.f : 1.f / mass;
+    store4(p.out, p.dtype, (((size_t)b * p.seq + token) * p.heads + head) * p.c.dim + col, make_float4(y.x * inv, y.y * inv, y.z * inv, y.w * inv));
+}
+
+template <int NG, int R, int TERMS>
+__global__ void __launch_bounds__(A4_THREADS, NG* R <= 4 ? 2 : 1) attend4_kernel(const __grid_constant__ Attend4 p) {
+    using C = A4Cfg<NG, R, TERMS>;
+    using T = Tile4<NG>;
+    constexpr int D = C::D, Q = C::Q, S = C::STAGES;
+    extern __shared__ __align__(128) unsigned char a4_raw[];
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+    const int blocks = (p.rows + Q - 1) / Q, block = blockIdx.x / p.splits, split = blockIdx.x - block * p.splits;
+    const int hk = block / blocks, r0 = (block - hk * blocks) * Q, b = blockIdx.y;
+    pdl_wait();
+    pdl_trigger();
+
+    const int past = past_of(p.past, b, p.c.max_seq), last_row = min(r0 + Q, p.rows) - 1;
+    const int pos0 = past + r0 / p.group, pos1 = past + last_row / p.group;  // positions of the block's first and last row
+    const int seen0 = first_visible(pos0, 0, p.window), seen1 = min(pos1, p.c.max_seq - 1);  // what some row sees
+    const int tile0 = seen0 / 16, tiles = max(seen1 / 16 + 1 - tile0, 0);
+    const int per = (tiles + p.splits - 1) / p.splits;
+    const int first = tile0 + split * per + warp, end = min(tile0 + (split + 1) * per, tile0 + tiles);
+    const T source(p.c, ((size_t)b * p.c.kv_heads + hk) * p.c.max_seq, lane);
+    unsigned char* ring = a4_raw + C::RING + warp * S * T::BYTES;
+    const uint32_t ring_at = (uint32_t)__cvta_generic_to_shared(ring);
+#pragma unroll
+    for (int s = 0; s < S - 1; ++s) {
+        if (first + s * A4_WARPS < end) source.fetch(first + s * A4_WARPS, ring_at + s * T::BYTES, lane);
+        copy_commit();
+    }
+
+    // ---- queries: warp j makes the operands of group j
+    uint4* frags = reinterpret_cast<uint4*>(a4_raw + C::FRAG);  // [j][term][h][lane]
+    float(*tops)[Q] = reinterpret_cast<float(*)[Q]>(a4_raw + C::TOPS);
+    float(*sums)[Q] = reinterpret_cast<float(*)[Q]>(a4_raw + C::SUMS);
+    float qv[R][8], fa[R][2];
+    int lo[R][2], hi[R][2];  // visible positions of query rows 2 t and 2 t + 1 (+ 8 h)
+#pragma unroll
+    for (int h = 0; h < R; ++h) {
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+            const int row = r0 + 8 * h + 2 * t + e, pos = past + min(row, last_row) / p.group;
+            lo[h][e] = first_visible(pos, 0, p.window);
+            hi[h][e] = min(pos, p.c.max_seq - 1);  // (rows past the last one repeat it, and are not kept)
+        }
+        if (warp < NG) {
+            const int row = min(r0 + g + 8 * h, last_row), token = row / p.group, head = hk * p.group + row - token * p.group;
+            const size_t at = (size_t)b * p.qb + (size_t)token * p.qs + (size_t)head * p.qh + 32 * warp + 8 * t;
+            if (p.dtype == ROTOR_B200_F32)
+                load8(static_cast<const float*>(p.q) + at, p.wide, qv[h]);
+            else if (p.dtype == ROTOR_B200_BF16)
+                load8(static_cast<const __nv_bfloat16*>(p.q) + at, p.wide, qv[h]);
+            else
+                load8(static_cast<const __half*>(p.q) + at, p.wide, qv[h]);
+            float top = 0.f, sum = 0.f;
+#pragma unroll
+            for (int n = 0; n < 8; ++n) {
+                top = fmaxf(top, fabsf(qv[h][n]));
+                sum += qv[h][n];
+            }
+#pragma unroll
+            for (int o = 1; o < 4; o <<= 1) {
+                top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+                sum += __shfl_xor_sync(0xffffffffu, sum, o);
+            }
+            if (t == 0) {
+                tops[warp][g + 8 * h] = top;
+                sums[warp][g + 8 * h] = sum;
+            }
+        }
+    }
+    __syncthreads();
+    uint32_t sum_hi[R], sum_lo[R];  // operands: sums of the queries over the groups' columns, as two terms
+#pragma unroll
+    for (int h = 0; h < R; ++h) {
+        float top = 0.f;
+#pragma unroll
+        for (int j = 0; j < NG; ++j) top = fmaxf(top, tops[j][g + 8 * h]);
+        // a power of two that takes the row's largest value to 2^14 .. 2^15 (none for rows of zeros, infinities and NaN)
+        const int e = (__float_as_int(top) >> 23) - 127;
+        const int up = top > 0.f && e < 128 ? min(14 - e, 100) : 0;
+        const float fs = __int_as_float((127 + up) << 23), back = p.scale2 * __int_as_float((127 - up) << 23);
+        fa[h][0] = __shfl_sync(0xffffffffu, back, 8 * t);
+        fa[h][1] = __shfl_sync(0xffffffffu, back, 8 * t + 4);
+        if (warp < NG) {
+            float x[8];
+#pragma unroll
+            for (int n = 0; n < 8; ++n) x[n] = qv[h][n] * (n & 1 ? fs * 0.0625f : fs);
+#pragma unroll
+            for (int term = 0; term < TERMS; ++term) {
+                const uint4 f = make_uint4(pack_half(x[0], x[4]), pack_half(x[2], x[6]), pack_half(x[1], x[5]), pack_half(x[3], x[7]));
+                frags[((warp * TERMS + term) * R + h) * 32 + lane] = f;
+                if (TERMS > 1) {
+                    const float2 a = half2_of(f.x), c = half2_of(f.y), d = half2_of(f.z), w = half2_of(f.w);
+                    x[0] -= a.x, x[4] -= a.y, x[2] -= c.x, x[6] -= c.y, x[1] -= d.x, x[5] -= d.y, x[3] -= w.x, x[7] -= w.y;
+                }
+            }
+        }
+        // up to four groups: lanes 0 and 1 of a quad hold the first terms of two groups, 2 and 3 the second ones
+        const int pair = NG > 4 ? 2 * t : 2 * (t & 1);
+        const float f6 = fs * 0.015625f;  // (the sum of 32 columns is up to 2^20 and has to fit as well)
+        const float s0 = pair < NG ? sums[pair][g + 8 * h] * f6 : 0.f, s1 = pair + 1 < NG ? sums[pair + 1][g + 8 * h] * f6 : 0.f;
+        const uint32_t big = pack_half(s0, s1);
+        const float2 bf = half2_of(big);
+        const uint32_t rest = pack_half(s0 - bf.x, s1 - bf.y);
+        sum_hi[h] = NG > 4 || t < 2 ? big : rest;
+        sum_lo[h] = NG > 4 ? rest : 0u;
+    }
+    __syncthreads();
+    uint4 kept[C::KEEP ? NG * TERMS * R : 1];
+    if constexpr (C::KEEP) {
+#pragma unroll
+        for (int i = 0; i < NG * TERMS * R; ++i) kept[i] = frags[i * 32 + lane];
+    }
+    auto frag = [&](int j, int term, int h) {
+        const int i = (j * TERMS + term) * R + h;
+        return C::KEEP ? kept[C::KEEP ? i : 0] : frags[i * 32 + lane];
+    };
+
+    float shift[R][2], o[R][2 * NG][4], rest[R][4];  // rest: row g: sum of p m of group g; row 8 (lanes 0 .. 3): sum of p
+    float lift = A4_LIFT;
+#pragma unroll
+    for (int h = 0; h < R; ++h) {
+        shift[h][0] = shift[h][1] = A4_LOW;
+#pragma unroll
+        for (int n = 0; n < 4; ++n) {
+            rest[h][n] = 0.f;
+#pragma unroll
+            for (int i = 0; i < 2 * NG; ++i) o[h][i][n] = 0.f;
+        }
+    }
+    auto rescale = [&](int h, float a0, float a1) {
+#pragma unroll
+        for (int i = 0; i < 2 * NG; ++i) o[h][i][0] *= a0, o[h][i][1] *= a1, o[h][i][2] *= a0, o[h][i][3] *= a1;
+        rest[h][0] *= a0, rest[h][1] *= a1, rest[h][2] *= a0, rest[h][3] *= a1;
+    };
+    const int key_row = 4 * (g >> 1) + (g & 1);  // rows g and g + 8 of the key operand: this position of the tile, and two more
+    // tiles that every row sees whole
+    const int inner0 = (first_visible(pos1, 0, p.window) + 15) / 16, inner1 = (min(pos0, p.c.max_seq - 1) + 1) / 16;
+    int stage = 0;
+    for (int tile = first; tile < end; tile += A4_WARPS) {
+        copy_wait<S - 2>();
+        __syncwarp();
+        {
+            const int ahead = tile + (S - 1) * A4_WARPS;
+            const int into = stage == 0 ? S - 1 : stage - 1;
+            if (ahead < end) source.fetch(ahead, ring_at + into * T::BYTES, lane);
+            copy_commit();
+        }
+        const unsigned char* x = ring + stage * T::BYTES;
+        stage = stage == S - 1 ? 0 : stage + 1;
+
+        // ---- scores of 16 positions x 8 R rows: lane's positions key_row and key_row + 2, rows 2 t and 2 t + 1 (+ 8 h)
+        float sc[R][4];
+        {
+            Bytes<4 * NG> k0, k1;
+            Bytes<2 * NG> s0, s1;
+            k0.load(x + key_row * (16 * NG) + t * (4 * NG));
+            k1.load(x + (key_row + 2) * (16 * NG) + t * (4 * NG));
+            s0.load(x + T::KS + key_row * (2 * NG));
+            s1.load(x + T::KS + (key_row + 2) * (2 * NG));
+            uint32_t km[2];
+            const int pair = NG > 4 ? 2 * t : 2 * (t & 1);
+#pragma unroll
+            for (int u = 0; u < 2; ++u) {
+                const unsigned short* m = reinterpret_cast<const unsigned short*>(x + T::KM + (key_row + 2 * u) * (2 * NG)) + pair;
+                if constexpr (NG % 2 == 0)
+                    km[u] = pair < NG ? *reinterpret_cast<const uint32_t*>(m) : 0u;
+                else
+                    km[u] = (pair < NG ? m[0] : 0u) | (uint32_t)(pair + 1 < NG ? m[1] : 0u) << 16;
+            }
+#pragma unroll
+            for (int h = 0; h < R; ++h) {
+                float low[4] = {0.f, 0.f, 0.f, 0.f};
+                a4_mma(low, km[0], km[1], NG > 4 ? km[0] : 0u, NG > 4 ? km[1] : 0u, sum_hi[h], sum_lo[h]);
+#pragma unroll
+                for (int i = 0; i < 4; ++i) sc[h][i] = low[i] * 64.f;
+            }
+#pragma unroll
+            for (int j = 0; j < NG; ++j) {
+                const uint32_t w0 = k0.w[j], w1 = k1.w[j];
+                const float f0 = s0.half_at(j) * 16777216.f, f1 = s1.half_at(j) * 16777216.f;
+#pragma unroll
+                for (int h = 0; h < R; ++h) {
+                    float acc[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                    for (int term = TERMS - 1; term >= 0; --term) {
+                        const uint4 f = frag(j, term, h);
+                        a4_mma(acc, w0 & 0x000f000fu, w1 & 0x000f000fu, w0 >> 8 & 0x000f000fu, w1 >> 8 & 0x000f000fu, f.x, f.y);
+                        a4_mma(acc, w0 & 0x00f000f0u, w1 & 0x00f000f0u, w0 >> 8 & 0x00f000f0u, w1 >> 8 & 0x00f000f0u, f.z, f.w);
+                    }
+                    sc[h][0] = fmaf(f0, acc[0], sc[h][0]);
+                    sc[h][1] = fmaf(f0, acc[1], sc[h][1]);
+                    sc[h][2] = fmaf(f1, acc[2], sc[h][2]);
+                    sc[h][3] = fmaf(f1, acc[3], sc[h][3]);
+                }
+            }
+        }
+#pragma unroll
+        for (int h = 0; h < R; ++h)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) sc[h][i] *= fa[h][i & 1];
+
+        // ---- the values' s; above 2 (bit 14 of a float16) the weights have to be kept smaller
+        Bytes<8 * NG> vs;
+        vs.load(x + T::VS + t * (8 * NG));
+        if (tile < inner0 || tile >= inner1) {
+#pragma unroll
+            for (int h = 0; h < R; ++h)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const int pos = tile * 16 + key_row + (i & 2);
+                    if (pos < lo[h][i & 1] || pos > hi[h][i & 1]) sc[h][i] = -INFINITY;
+                }
+            // (what lies in places that no row sees does not count)
+            const int at = tile * 16 + 4 * t;
+            auto seen = [&](int pos) { return pos >= seen0 && pos <= seen1 ? 0xffffu : 0u; };
+            const uint32_t m01 = seen(at) | seen(at + 1) << 16, m23 = seen(at + 2) | seen(at + 3) << 16;
+#pragma unroll
+            for (int j = 0; j < NG; ++j) {
+                vs.w[2 * j] &= m01;
+                vs.w[2 * j + 1] &= m23;
+            }
+        }
+        uint32_t any = 0;
+#pragma unroll
+        for (int i = 0; i < 2 * NG; ++i) any |= vs.w[i];
+        bool higher = false;
+#pragma unroll
+        for (int h = 0; h < R; ++h)
+#pragma unroll
+            for (int e = 0; e < 2; ++e) higher |= fmaxf(sc[h][e], sc[h][e + 2]) > shift[h][e] + (A4_SLACK + lift);
+        if (__any_sync(0xffffffffu, higher || (any & 0x40004000u))) {
+            float most = 0.f;
+#pragma unroll
+            for (int i = 0; i < 4 * NG; ++i) most = fmaxf(most, vs.half_at(i));
+            most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 1));
+            most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 2));
+            const int exponent = (__float_as_int(most) >> 23) - 127;
+            const float now = fminf(lift, A4_LIFT - (float)max(exponent, 0));
+#pragma unroll
+            for (int h = 0; h < R; ++h) {
+                float alpha[2];
+#pragma unroll
+                for (int e = 0; e < 2; ++e) {
+                    float m = fmaxf(sc[h][e], sc[h][e + 2]);
+#pragma unroll
+                    for (int n = 4; n < 32; n <<= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, n));
+                    m = fmaxf(shift[h][e] + (lift - now), m - now);
+                    alpha[e] = a4_exp2(shift[h][e] - m);
+                    shift[h][e] = m;
+                }
+                rescale(h, alpha[0], alpha[1]);
+            }
+            lift = now;
+        }
+
+        // ---- weights, turned into the operand of the second product: row g of the queries, positions 4 t .. 4 t + 3
+        uint32_t pw[R][TERMS][2];
+#pragma unroll
+        for (int h = 0; h < R; ++h) {
+#pragma unroll
+            for (int u = 0; u < 2; ++u) {
+                const float e0 = a4_exp2(sc[h][2 * u] - shift[h][0]), e1 = a4_exp2(sc[h][2 * u + 1] - shift[h][1]);
+                const uint32_t w = pack_half(e0, e1);
+                pw[h][0][u] = turned(w);
+                if (TERMS > 1) {
+                    const float2 f = half2_of(w);
+                    pw[h][TERMS - 1][u] = turned(pack_half(e0 - f.x, e1 - f.y));
+                }
+            }
+        }
+
+        // ---- sums over the positions
+        {
+            Bytes<8> vm;
+            vm.w[0] = vm.w[1] = 0u;
+            if (g < NG) vm.load(x + T::VM + t * (8 * NG) + g * 8);
+            const uint32_t ones = g == 0 ? 0x3c003c00u : 0u;
+#pragma unroll
+            for (int h = 0; h < R; ++h) {
+                float d[4] = {0.f, 0.f, 0.f, 0.f};
+                if constexpr (TERMS > 1) {
+                    a4_mma(d, vm.w[0], ones, vm.w[1], ones, pw[h][1][0], pw[h][1][1]);
+                    a4_mma(d, vm.w[0], ones, vm.w[1], ones, pw[h][0][0], pw[h][0][1]);
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) rest[h][i] += d[i];
+                } else {
+                    a4_mma(rest[h], vm.w[0], ones, vm.w[1], ones, pw[h][0][0], pw[h][0][1]);
+                }
+            }
+        }
+#pragma unroll
+        for (int j = 0; j < NG; ++j) {
+            Bytes<8> y;  // words of positions 4 t, 4 t + 1 and 4 t + 2, 4 t + 3
+            y.load(x + T::V + 2 * value_at(NG, j, 0, 0) + lane * (j < NG / 2 * 2 ? 16 : 8));
+            const uint32_t a = y.w[0], c = y.w[1];
+#pragma unroll
+            for (int h = 0; h < R; ++h) {
+                const __half2 s0 = as_half2(vs.w[2 * j]), s1 = as_half2(vs.w[2 * j + 1]);
+                const __half2 w0 = __hmul2(as_half2(pw[h][0][0]), s0), w1 = __hmul2(as_half2(pw[h][0][1]), s1);
+                if constexpr (TERMS > 1) {
+                    // what the rounding of p s left out, and the second term of p
+                    const __half2 l0 = __hfma2(as_half2(pw[h][1][0]), s0, __hfma2(as_half2(pw[h][0][0]), s0, __hneg2(w0)));
+                    const __half2 l1 = __hfma2(as_half2(pw[h][1][1]), s1, __hfma2(as_half2(pw[h][0][1]), s1, __hneg2(w1)));
+                    float d[4] = {0.f, 0.f, 0.f, 0.f}, d2[4] = {0.f, 0.f, 0.f, 0.f};
+                    a4_mma(d, a & 0x000f000fu, a & 0x00f000f0u, c & 0x000f000fu, c & 0x00f000f0u, as_word(l0), as_word(l1));
+                    a4_mma(d2, a >> 8 & 0x000f000fu, a >> 8 & 0x00f000f0u, c >> 8 & 0x000f000fu, c >> 8 & 0x00f000f0u, as_word(l0), as_word(l1));
+                    a4_mma(d, a & 0x000f000fu, a & 0x00f000f0u, c & 0x000f000fu, c & 0x00f000f0u, as_word(w0), as_word(w1));
+                    a4_mma(d2, a >> 8 & 0x000f000fu, a >> 8 & 0x00f000f0u, c >> 8 & 0x000f000fu, c >> 8 & 0x00f000f0u, as_word(w0), as_word(w1));
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        o[h][2 * j][i] += d[i];
+                        o[h][2 * j + 1][i] += d2[i];
+                    }
+                } else {
+                    a4_mma(o[h][2 * j], a & 0x000f000fu, a & 0x00f000f0u, c & 0x000f000fu, c & 0x00f000f0u, as_word(w0), as_word(w1));
+                    a4_mma(o[h][2 * j + 1], a >> 8 & 0x000f000fu, a >> 8 & 0x00f000f0u, c >> 8 & 0x000f000fu, c >> 8 & 0x00f000f0u, as_word(w0),
+                           as_word(w1));
+                }
+            }
+        }
+    }
+
+    // ---- the warps' sums are joined in shared memory
+    copy_wait<0>();
+    __syncthreads();  // (every warp has read its last tile: the sums lie over the rings)
+    float* all = reinterpret_cast<float*>(a4_raw + C::O);  // [warp][row][OS]
+    float(*shifts)[Q] = reinterpret_cast<float(*)[Q]>(a4_raw + C::SHIFT);
+    float(*masses)[Q] = reinterpret_cast<float(*)[Q]>(a4_raw + C::MASS);
+#pragma unroll
+    for (int h = 0; h < R; ++h) {
+        const int r = 8 * h + 2 * t;
+        if (g == 0) {
+            shifts[warp][r] = shift[h][0];
+            shifts[warp][r + 1] = shift[h][1];
+            masses[warp][r] = rest[h][2];
+            masses[warp][r + 1] = rest[h][3];
+        }
+        float* to = all + (warp * Q + r) * C::OS + 4 * g;
+#pragma unroll
+        for (int j = 0; j < NG; ++j) {
+            // columns 32 j + 4 g .. + 3; sums of codes four bits higher are 16 times too large
+            const float l0 = __shfl_sync(0xffffffffu, rest[h][0], 4 * j + t), l1 = __shfl_sync(0xffffffffu, rest[h][1], 4 * j + t);
+            constexpr float c0 = 16777216.f, c1 = 1048576.f;
+            const float(&a)[4] = o[h][2 * j], (&c)[4] = o[h][2 * j + 1];
+            *reinterpret_cast<float4*>(to + 32 * j) = make_float4(fmaf(a[0], c0, l0), fmaf(a[2], c1, l0), fmaf(c[0], c0, l0), fmaf(c[2], c1, l0));
+            *reinterpret_cast<float4*>(to + C::OS + 32 * j) =
+                make_float4(fmaf(a[1], c0, l1), fmaf(a[3], c1, l1), fmaf(c[1], c0, l1), fmaf(c[3], c1, l1));
+        }
+    }
+    __syncthreads();
+    for (int idx = threadIdx.x; idx < Q * (D / 4); idx += A4_THREADS) {
+        const int r = idx / (D / 4), c4 = idx - r * (D / 4), row = r0 + r;
+        if (row >= p.rows) break;
+        float top = A4_LOW, total = 0.f;
+#pragma unroll
+        for (int w = 0; w < A4_WARPS; ++w) top = fmaxf(top, shifts[w][r]);
+        float4 y = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+        for (int w = 0; w < A4_WARPS; ++w) {
+            const float f = a4_exp2(shifts[w][r] - top);
+            const float4 v = *reinterpret_cast<const float4*>(all + (w * Q + r) * C::OS + 4 * c4);
+            total = fmaf(f, masses[w][r], total);
+            y.x = fmaf(f, v.x, y.x), y.y = fmaf(f, v.y, y.y), y.z = fmaf(f, v.z, y.z), y.w = fmaf(f, v.w, y.w);
+        }
+        if (p.splits == 1) {
+            finish4(p, b, hk, row, 4 * c4, y, total, top);
+            continue;
+        }
+        float* part = p.part + (((size_t)(b * p.c.kv_heads + hk) * p.rows + row) * p.splits + split) * (D + 4);
+        *reinterpret_cast<float4*>(part + 4 * c4) = y;
+        if (c4 == 0) *reinterpret_cast<float2*>(part + D) = make_float2(top, total);
+    }
+}
+
+// Joins the splits of a query row: a warp per row.
 __global__ void __launch_bounds__(32) attend4_join_kernel(const __grid_constant__ Attend4 p) {
     pdl_wait();
     pdl_trigger();
-    const int D = p.c.dim, row = blockIdx.x, hk = blockIdx.y, b = blockIdx.z;
+    const int D = p.c.dim, hk = blockIdx.x / p.rows, row = blockIdx.x - hk * p.rows, b = blockIdx.y;
     const float* part = p.part + ((size_t)(b * p.c.kv_heads + hk) * p.rows + row) * p.splits * (D + 4);
-    const int token = row / p.group, head = hk * p.group + row - token * p.group;
-    float top = -INFINITY;
-    for (int s = 0; s < p.splits; ++s) top = fmaxf(top, __ldcg(part + (size_t)s * (D + 4) + D));
-    const float sink = p.sinks ? __ldg(p.sinks + head) * 1.4426950408889634f : -INFINITY;
-    const float ref = fmaxf(top, sink) == -INFINITY ? 0.f : fmaxf(top, sink);
+    float top = A4_LOW;
+    for (int s = threadIdx.x; s < p.splits; s += 32) top = fmaxf(top, __ldcg(part + (size_t)s * (D + 4) + D));
+    top = warp_max(top);
     for (int c = 4 * threadIdx.x; c < D; c += 128) {
-        float total = a4_exp2(sink - ref);
+        float total = 0.f;
         float4 y = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 4
         for (int s = 0; s < p.splits; ++s) {
             const float* q = part + (size_t)s * (D + 4);
             const float2 ml = __ldcg(reinterpret_cast<const float2*>(q + D));
             const float4 v = __ldcg(reinterpret_cast<const float4*>(q + c));
-            const float f = a4_exp2(ml.x - ref);
+            const float f = a4_exp2(ml.x - top);
             total = fmaf(f, ml.y, total);
             y.x = fmaf(f, v.x, y.x), y.y = fmaf(f, v.y, y.y), y.z = fmaf(f, v.z, y.z), y.w = fmaf(f, v.w, y.w);
         }
-        const float inv = total == 0.f ? 0.f : 1.f / total;  // (a row that sees no position: zeros)
-        store4(p.out, p.dtype, (((size_t)b * p.seq + token) * p.heads + head) * D + c, make_float4(y.x * inv, y.y * inv, y.z * inv, y.w * inv));
+        finish4(p, b, hk, row, c, y, total, top);
     }
 }
 
@@ -471,21 +591,21 @@ static Attend4Plan attend4_plan(const Cache4View& c, int rows, int reach) {
     if (splits > most) splits = most;
     if (splits < 1) splits = 1;
     a.splits = (int)splits;
-    a.part_bytes = (size_t)c.batch * c.kv_heads * rows * splits * (c.dim + 4) * sizeof(float);
+    a.part_bytes = splits == 1 ? 16 : (size_t)c.batch * c.kv_heads * rows * splits * (c.dim + 4) * sizeof(float);
     return a;
 }
 
 template <int NG, int R, int TERMS>
 static int attend4_go(const Attend4& a, const Attend4Plan& plan, cudaStream_t st) {
-    constexpr size_t s1 = sizeof(Attend4Smem<NG, R>), s2 = sizeof(Attend4Query<NG, R, TERMS>), smem = s1 > s2 ? s1 : s2;
+    constexpr int smem = A4Cfg<NG, R, TERMS>::SMEM;
     static PerDevice<bool> once;
     if (!once.here()) {
-        RB_CUDA(cudaFuncSetAttribute(attend4_kernel<NG, R, TERMS>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+        RB_CUDA(cudaFuncSetAttribute(attend4_kernel<NG, R, TERMS>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
         once.here() = true;
     }
-    const dim3 grid(a.c.kv_heads * ((a.rows + plan.per_block - 1) / plan.per_block), a.splits, a.c.batch);
-    if (const int e = launch_chained(attend4_kernel<NG, R, TERMS>, grid, A4_THREADS, smem, st, 1, a)) return e;
-    return launch_chained(attend4_join_kernel, dim3(a.rows, a.c.kv_heads, a.c.batch), 32, 0, st, 1, a);
+    const dim3 grid(a.c.kv_heads * ((a.rows + plan.per_block - 1) / plan.per_block) * a.splits, a.c.batch);
+    const int e = launch_chained(attend4_kernel<NG, R, TERMS>, grid, A4_THREADS, smem, st, 1, a);
+    return e || a.splits == 1 ? e : launch_chained(attend4_join_kernel, dim3(a.rows * a.c.kv_heads, a.c.batch), 32, 0, st, 1, a);
 }
 
 template <int NG>

@@ -10,7 +10,7 @@ import ctypes as C
 
 from . import abi
 from .abi import RotorB200Error, check, lib
-from .ops import on_device, type_code
+from .ops import on_device, reorder_states, type_code
 
 GROUP = 32
 DIMS = (32, 64, 96, 128, 192, 256)
@@ -41,8 +41,14 @@ class Cache4:
         return self.k_codes, self.v_codes, self.k_step, self.k_least, self.v_step, self.v_least
 
     def states(self):
-        """For ``ops.reorder_states``: the tensors, each with the axis its positions run along."""
+        """For ``ops.reorder_states``: the tensors, each with the axis its positions run along.  Positions lie in tiles of 16: a
+        ``length`` given with them has to be rounded up to that (``reorder`` does it)."""
         return [(t, 2) for t in self._tensors()]
+
+    def reorder(self, beams, length=None):
+        """``ops.reorder_states`` of this cache: sequence b * width + w becomes what b * width + beams[b, w] was, in its first
+        ``length`` positions (all of them unless given)."""
+        reorder_states(self.states(), beams, None if length is None else min(-(-length // 16) * 16, self.max_seq))
 
     def _past(self, past, seq):
         """(number, address of the lengths or None), checked."""
