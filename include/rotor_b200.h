@@ -460,10 +460,9 @@ int rotor_b200_reorder_states(const rotor_b200_state* states, int n, const int64
  *  attend: q `dtype` [batch][seq][heads][dim] sits at positions past .. past + seq - 1 and sees cached positions j <= its own,
  *    with window > 0 those with (own - j) < window.  Softmax of scale * q . k, whose denominator holds exp(sinks[head]) as well
  *    (sinks float32 [heads] or NULL); query head h reads KV head h / (heads / kv_heads).  out: `dtype` [batch][seq][heads][dim],
- *    16-byte aligned.  A query that sees no position gives zeros.  `longest`: with past_len, a bound of what a sequence holds
- *    that the work is divided by (results do not depend on its being right); without, not read.  workspace:
- *    rotor_b200_cache4_attend_workspace_bytes bytes with `longest` = past where past_len is NULL, 16-byte aligned, contents of no
- *    matter. */
+ *    16-byte aligned.  A query that sees no position gives zeros.  `longest`: with past_len, the most that a sequence holds, by which the
+ *    work is divided; longer lengths are taken as it.  Without, not read but for the size of the workspace: 16-byte
+ *    aligned, contents of no matter, rotor_b200_cache4_attend_workspace_bytes bytes with `longest` = past where past_len is NULL. */
 typedef struct rotor_b200_cache4 {
     int32_t batch, kv_heads, max_seq, dim;
     uint8_t *k_codes, *v_codes;
@@ -472,7 +471,7 @@ typedef struct rotor_b200_cache4 {
 int rotor_b200_cache4_append(const rotor_b200_cache4* cache, const void* k, const void* v, int dtype, const int64_t* k_strides_host,
                              const int64_t* v_strides_host, int seq, int past, const int32_t* past_len, void* stream);
 int rotor_b200_cache4_read(const rotor_b200_cache4* cache, int begin, int end, void* k, void* v, int dtype, void* stream);
-size_t rotor_b200_cache4_attend_workspace_bytes(const rotor_b200_cache4* cache, int heads, int seq, int longest, int window);
+size_t rotor_b200_cache4_attend_workspace_bytes(const rotor_b200_cache4* cache, int dtype, int heads, int seq, int longest, int window);
 int rotor_b200_cache4_attend(const rotor_b200_cache4* cache, const void* q, int dtype, const int64_t* q_strides_host, int heads, int seq,
                              int past, const int32_t* past_len, int longest, float scale, int window, const float* sinks, void* out,
                              void* workspace, size_t workspace_bytes, void* stream);

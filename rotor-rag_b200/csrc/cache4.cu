@@ -93,7 +93,7 @@ __global__ void __launch_bounds__(C4_THREADS) cache4_store_kernel(const __grid_c
             word |= (uint32_t)(int)fmin(fmax(rint(q), 0.0), 15.0) << (4 * n);
         }
     }
-    const int pos = past_of(p.past, b, p.c.max_seq) + (int)i;
+    const int pos = past_of(p.past, b) + (int)i;
     if (!on || pos >= p.c.max_seq) return;
     const Place w(p.c, part, b, h, pos, c8);
     if (part == 0) {
@@ -114,9 +114,13 @@ struct Cache4Load {
     int begin, span;
     uint32_t units;  // kv_heads * span * dim / 8
     FastDiv per_row, positions;
+    // rows for a prompt
+    int seq, window;
+    Past past;
+    int* past_out;
 };
 
-template <typename T>
+template <typename T, bool PROMPT>
 __global__ void __launch_bounds__(C4_THREADS) cache4_load_kernel(const __grid_constant__ Cache4Load p) {
     pdl_wait();
     pdl_trigger();
@@ -125,12 +129,30 @@ __global__ void __launch_bounds__(C4_THREADS) cache4_load_kernel(const __grid_co
     if (u >= p.units) return;
     const uint32_t row = p.per_row.div(u), c8 = u - row * p.per_row.d;
     const uint32_t h = p.positions.div(row), pos = p.begin + row - h * p.positions.d;
+    bool there = true;
+    if constexpr (PROMPT) {
+        // the attention reads tiles of 128 positions from the first one its first query sees: a head's rows end in zeros, and so begin
+        // the rows that a tile at the end of the head before reaches into
+        const int past = past_of(p.past, b), limit = min(past + p.seq, p.c.max_seq);
+        if (p.past_out && u == 0 && part == 0) p.past_out[b] = past;
+        if ((int)pos >= limit + 128 || ((int)pos < first_visible(past, 0, p.window) && pos >= 128)) return;
+        there = (int)pos < limit;
+    }
     float x[8];
-    const Place w(p.c, part, b, h, pos, c8);
-    const uint32_t word = part == 0 ? *reinterpret_cast<const uint32_t*>(w.codes) : w.codes[0] | (uint32_t)w.codes[w.next] << 16;
-    const float s = __half2float(p.c.step[part][w.group]), m = __half2float(p.c.least[part][w.group]);
+    uint32_t word = 0;
+    float s = 0.f, m = 0.f;
+    if (there) {
+        const Place w(p.c, part, b, h, pos, c8);
+        word = part == 0 ? *reinterpret_cast<const uint32_t*>(w.codes) : w.codes[0] | (uint32_t)w.codes[w.next] << 16;
+        s = __half2float(p.c.step[part][w.group]);
+        m = __half2float(p.c.least[part][w.group]);
+    }
 #pragma unroll
     for (int n = 0; n < 8; ++n) x[n] = fmaf((float)(word >> (4 * n) & 15u), s, m);
+    if constexpr (PROMPT) {
+#pragma unroll
+        for (int n = 0; n < 8; ++n) x[n] = fminf(x[n], C4_MOST);  // (m + 15 s may lie a rounding above the largest float16)
+    }
     store8(static_cast<T*>(p.dst[part]) + (((size_t)b * p.c.kv_heads + h) * p.span + (pos - p.begin)) * p.c.dim + c8 * 8, x);
 }
 
@@ -157,24 +179,29 @@ int cache4_view(const rotor_b200_cache4* c, Cache4View& v) {
     return ROTOR_B200_OK;
 }
 
-int launch_cache4_read(const Cache4Read& r, cudaStream_t st) {
-    const uint64_t units = (uint64_t)r.c.kv_heads * r.span * (r.c.dim / 8);
+static int load_units(Cache4Load& p) {
+    const uint64_t units = (uint64_t)p.c.kv_heads * p.span * (p.c.dim / 8);
     if (units > 0x7fffff00u) return ROTOR_B200_ERR_SHAPE;
-    Cache4Load p;
+    p.units = (uint32_t)units;
+    p.per_row = FastDiv(p.c.dim / 8);
+    p.positions = FastDiv(p.span);
+    return ROTOR_B200_OK;
+}
+
+int launch_cache4_expand(const Cache4Expand& r, cudaStream_t st) {
+    Cache4Load p = {};
     p.c = r.c;
     p.dst[0] = r.k;
     p.dst[1] = r.v;
-    p.begin = r.begin;
     p.span = r.span;
-    p.units = (uint32_t)units;
-    p.per_row = FastDiv(r.c.dim / 8);
-    p.positions = FastDiv(r.span);
-    const dim3 grid((p.units + C4_THREADS - 1) / C4_THREADS, r.c.batch, 2);
-    switch (r.dtype) {
-        case ROTOR_B200_F32: return launch_chained(cache4_load_kernel<float>, grid, C4_THREADS, 0, st, 1, p);
-        case ROTOR_B200_BF16: return launch_chained(cache4_load_kernel<__nv_bfloat16>, grid, C4_THREADS, 0, st, 1, p);
-        default: return launch_chained(cache4_load_kernel<__half>, grid, C4_THREADS, 0, st, 1, p);
-    }
+    p.seq = r.seq;
+    p.window = r.window;
+    p.past = r.past;
+    p.past_out = r.past_out;
+    if (const int e = load_units(p)) return e;
+    const dim3 grid((p.units + C4_THREADS - 1) / C4_THREADS, p.c.batch, 2);
+    return r.half ? launch_chained(cache4_load_kernel<__half, true>, grid, C4_THREADS, 0, st, 1, p)
+                  : launch_chained(cache4_load_kernel<__nv_bfloat16, true>, grid, C4_THREADS, 0, st, 1, p);
 }
 
 }  // namespace rb
@@ -203,7 +230,7 @@ int rotor_b200_cache4_append(const rotor_b200_cache4* cache, const void* k, cons
     }
     const uint64_t units = (uint64_t)seq * p.c.kv_heads * (p.c.dim / 8);
     if (units > 0x7fffff00u) return ROTOR_B200_ERR_SHAPE;
-    p.past = Past{past_len, past};
+    p.past = Past{past_len, past, p.c.max_seq};
     p.units = (uint32_t)units;
     p.per_row = FastDiv(p.c.dim / 8);
     p.heads = FastDiv(p.c.kv_heads);
@@ -217,16 +244,22 @@ int rotor_b200_cache4_append(const rotor_b200_cache4* cache, const void* k, cons
 }
 
 int rotor_b200_cache4_read(const rotor_b200_cache4* cache, int begin, int end, void* k, void* v, int dtype, void* stream) {
-    Cache4Read r = {};
-    if (const int e = cache4_view(cache, r.c)) return e;
-    RB_REQUIRE(k && v && dtype >= ROTOR_B200_F32 && dtype <= ROTOR_B200_F16 && begin >= 0 && end > begin && end <= r.c.max_seq);
+    Cache4Load p = {};
+    if (const int e = cache4_view(cache, p.c)) return e;
+    RB_REQUIRE(k && v && dtype >= ROTOR_B200_F32 && dtype <= ROTOR_B200_F16 && begin >= 0 && end > begin && end <= p.c.max_seq);
     RB_REQUIRE((((uintptr_t)k | (uintptr_t)v) & 15) == 0);
-    r.k = k;
-    r.v = v;
-    r.dtype = dtype;
-    r.begin = begin;
-    r.span = end - begin;
-    return launch_cache4_read(r, as_stream(stream));
+    p.dst[0] = k;
+    p.dst[1] = v;
+    p.begin = begin;
+    p.span = end - begin;
+    if (const int e = load_units(p)) return e;
+    const dim3 grid((p.units + C4_THREADS - 1) / C4_THREADS, p.c.batch, 2);
+    const cudaStream_t st = as_stream(stream);
+    switch (dtype) {
+        case ROTOR_B200_F32: return launch_chained(cache4_load_kernel<float, false>, grid, C4_THREADS, 0, st, 1, p);
+        case ROTOR_B200_BF16: return launch_chained(cache4_load_kernel<__nv_bfloat16, false>, grid, C4_THREADS, 0, st, 1, p);
+        default: return launch_chained(cache4_load_kernel<__half, false>, grid, C4_THREADS, 0, st, 1, p);
+    }
 }
 
 }  // extern "C"

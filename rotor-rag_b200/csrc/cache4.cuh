@@ -44,14 +44,12 @@ struct FastDiv {
     __device__ __forceinline__ uint32_t div(uint32_t x) const { return (__umulhi(x, mul) + x) >> shift; }
 };
 
-// Where sequence b of a call starts: a number for all, or one per sequence in device memory.
+// Where sequence b of a call starts: a number for all, or one per sequence in device memory, taken as at most `most`.
 struct Past {
     const int* each;
-    int all;
+    int all, most;
 };
-__device__ __forceinline__ int past_of(const Past& p, int b, int max_seq) {
-    return p.each ? min(max(__ldcg(p.each + b), 0), max_seq) : p.all;
-}
+__device__ __forceinline__ int past_of(const Past& p, int b) { return p.each ? min(max(__ldcg(p.each + b), 0), p.most) : p.all; }
 
 __device__ __forceinline__ float type_load(const float* p) { return *p; }
 __device__ __forceinline__ float type_load(const __nv_bfloat16* p) { return __bfloat162float(*p); }
@@ -105,12 +103,15 @@ __device__ __forceinline__ void store8(__half* p, const float (&x)[8]) {
 int cache4_view(const rotor_b200_cache4* c, Cache4View& v);  // checks the description
 
 
-// The positions [begin, begin + span) of every sequence and head as dense rows [batch][kv_heads][span][dim] of `dtype`.
-struct Cache4Read {
+// The first `span` positions of every sequence and head as dense rows [batch][kv_heads][span][dim], bf16 or float16, as the prompt attention
+// of `seq` tokens reads them: zeros behind a sequence's last position, nothing where no query looks.  past goes to past_out as well.
+struct Cache4Expand {
     Cache4View c;
     void *k, *v;
-    int dtype, begin, span;
+    int half, span, seq, window;
+    Past past;
+    int* past_out;
 };
-int launch_cache4_read(const Cache4Read& r, cudaStream_t st);
+int launch_cache4_expand(const Cache4Expand& r, cudaStream_t st);
 
 }  // namespace rb

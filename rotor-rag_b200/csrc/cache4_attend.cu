@@ -190,7 +190,7 @@ __global__ void __launch_bounds__(A4_THREADS, NG* R <= 4 ? 2 : 1) attend4_kernel
     pdl_wait();
     pdl_trigger();
 
-    const int past = past_of(p.past, b, p.c.max_seq), last_row = min(r0 + Q, p.rows) - 1;
+    const int past = past_of(p.past, b), last_row = min(r0 + Q, p.rows) - 1;
     const int pos0 = past + r0 / p.group, pos1 = past + last_row / p.group;  // positions of the block's first and last row
     const int seen0 = first_visible(pos0, 0, p.window), seen1 = min(pos1, p.c.max_seq - 1);  // what some row sees
     const int tile0 = seen0 / 16, tiles = max(seen1 / 16 + 1 - tile0, 0);
@@ -575,14 +575,32 @@ __global__ void __launch_bounds__(32) attend4_join_kernel(const __grid_constant_
     }
 }
 
+// Query rows of a KV head from which 16-bit calls go to the prompt kernel: the cache's rows are made dense (bf16 or float16) in the workspace
+// first.
+constexpr int A4_PROMPT_ROWS = 192;
+
 struct Attend4Plan {
-    int splits, per_block;  // query rows of a block
-    size_t part_bytes;
+    bool prompt;
+    int span;                // prompt: dense rows of a head
+    size_t dense_bytes;      // of the keys, and of the values
+    int splits, per_block;   // else: CTAs that share a row's positions, query rows of a block
+    size_t bytes;            // of workspace
 };
 
-static Attend4Plan attend4_plan(const Cache4View& c, int rows, int reach) {
-    Attend4Plan a;
-    const int ng = c.dim / C4_GROUP;
+// For sequences that hold up to `longest` positions.
+static Attend4Plan attend4_plan(const Cache4View& c, int dtype, int heads, int seq, int longest, int window, bool wide) {
+    Attend4Plan a = {};
+    const int rows = seq * (heads / c.kv_heads), ng = c.dim / C4_GROUP;
+    const int held = (int)((long long)longest + seq < c.max_seq ? longest + seq : c.max_seq);
+    a.span = held;
+    a.prompt = wide && dtype != ROTOR_B200_F32 && rows >= A4_PROMPT_ROWS && prompt_attn_supported(c.batch, heads, c.kv_heads, c.dim, a.span) &&
+               (uint64_t)c.kv_heads * a.span * (c.dim / 8) <= 0x7fffff00u;
+    a.dense_bytes = round_up((size_t)c.batch * c.kv_heads * a.span * c.dim * 2, 256);
+    if (a.prompt) {
+        a.bytes = 2 * a.dense_bytes + (size_t)c.batch * sizeof(int);
+        return a;
+    }
+    const int reach = window > 0 && held > (long long)window + seq ? window + seq : held;  // what the queries see between them
     a.per_block = rows > 8 && ng <= 4 ? 16 : 8;
     const long long blocks = (long long)c.batch * c.kv_heads * ((rows + a.per_block - 1) / a.per_block);
     const long long tiles = (reach + 15) / 16 + 1;
@@ -591,7 +609,7 @@ static Attend4Plan attend4_plan(const Cache4View& c, int rows, int reach) {
     if (splits > most) splits = most;
     if (splits < 1) splits = 1;
     a.splits = (int)splits;
-    a.part_bytes = splits == 1 ? 16 : (size_t)c.batch * c.kv_heads * rows * splits * (c.dim + 4) * sizeof(float);
+    a.bytes = splits == 1 ? 16 : (size_t)c.batch * c.kv_heads * rows * splits * (c.dim + 4) * sizeof(float);
     return a;
 }
 
@@ -616,18 +634,12 @@ static int attend4_pick(const Attend4& a, const Attend4Plan& plan, cudaStream_t 
     return f32 ? attend4_go<NG, 1, 2>(a, plan, st) : attend4_go<NG, 1, 1>(a, plan, st);
 }
 
-static int attend4_check(const rotor_b200_cache4* cache, Cache4View& c, int heads, int seq, int longest) {
+static int attend4_check(const rotor_b200_cache4* cache, Cache4View& c, int dtype, int heads, int seq, int longest, int window) {
     if (const int e = cache4_view(cache, c)) return e;
-    RB_REQUIRE(heads > 0 && heads % c.kv_heads == 0 && seq > 0 && longest >= 0);
+    RB_REQUIRE(dtype >= ROTOR_B200_F32 && dtype <= ROTOR_B200_F16 && heads > 0 && heads % c.kv_heads == 0);
+    RB_REQUIRE(seq > 0 && seq <= c.max_seq && longest >= 0 && window >= 0);
     if ((long long)seq * (heads / c.kv_heads) > (1 << 24) || heads > 65535) return ROTOR_B200_ERR_SHAPE;
     return ROTOR_B200_OK;
-}
-
-// The most positions that the queries of a call see between them.
-static int attend4_reach(const Cache4View& c, int seq, int longest, int window) {
-    long long reach = (long long)longest + seq;
-    if (window > 0 && reach > (long long)window + seq) reach = (long long)window + seq;
-    return (int)(reach < c.max_seq ? reach : c.max_seq);
 }
 
 }  // namespace rb
@@ -636,42 +648,77 @@ using namespace rb;
 
 extern "C" {
 
-size_t rotor_b200_cache4_attend_workspace_bytes(const rotor_b200_cache4* cache, int heads, int seq, int longest, int window) {
+size_t rotor_b200_cache4_attend_workspace_bytes(const rotor_b200_cache4* cache, int dtype, int heads, int seq, int longest, int window) {
     Cache4View c;
-    if (attend4_check(cache, c, heads, seq, longest)) return 0;
-    return attend4_plan(c, seq * (heads / c.kv_heads), attend4_reach(c, seq, longest, window)).part_bytes;
+    if (attend4_check(cache, c, dtype, heads, seq, longest, window)) return 0;
+    const size_t a = attend4_plan(c, dtype, heads, seq, longest, window, true).bytes;
+    const size_t b = attend4_plan(c, dtype, heads, seq, longest, window, false).bytes;
+    return a > b ? a : b;
 }
 
 int rotor_b200_cache4_attend(const rotor_b200_cache4* cache, const void* q, int dtype, const int64_t* q_strides_host, int heads, int seq,
                              int past, const int32_t* past_len, int longest, float scale, int window, const float* sinks, void* out,
                              void* workspace, size_t workspace_bytes, void* stream) {
     Attend4 a;
-    if (const int e = attend4_check(cache, a.c, heads, seq, longest)) return e;
-    RB_REQUIRE(q && q_strides_host && out && workspace && dtype >= ROTOR_B200_F32 && dtype <= ROTOR_B200_F16 && past >= 0 && window >= 0);
-    RB_REQUIRE(seq <= a.c.max_seq && (past_len || past <= a.c.max_seq - seq));
+    if (const int e = attend4_check(cache, a.c, dtype, heads, seq, longest, window)) return e;
+    RB_REQUIRE(q && q_strides_host && out && workspace && past >= 0 && (past_len || past <= a.c.max_seq - seq));
     const int64_t* s = q_strides_host;
     const int size = dtype == ROTOR_B200_F32 ? 4 : 2;
     RB_REQUIRE(s[0] >= 0 && s[1] >= 0 && s[2] >= 0 && (uintptr_t)q % size == 0 && (((uintptr_t)out | (uintptr_t)workspace) & 15) == 0);
+    a.wide = (((uintptr_t)q | (uintptr_t)((s[0] | s[1] | s[2]) * size)) & 15) == 0;
+    a.past = Past{past_len, past, longest < a.c.max_seq ? longest : a.c.max_seq};
+    const Attend4Plan plan = attend4_plan(a.c, dtype, heads, seq, past_len ? longest : past, window, a.wide);
+    if (plan.bytes > workspace_bytes) return ROTOR_B200_ERR_WORKSPACE;
+    const cudaStream_t st = as_stream(stream);
+    if (plan.prompt) {
+        Cache4Expand x;
+        x.c = a.c;
+        x.k = workspace;
+        x.v = static_cast<char*>(workspace) + plan.dense_bytes;
+        x.half = dtype == ROTOR_B200_F16;
+        x.span = plan.span;
+        x.seq = seq;
+        x.window = window;
+        x.past = a.past;
+        x.past_out = reinterpret_cast<int*>(static_cast<char*>(workspace) + 2 * plan.dense_bytes);
+        if (const int e = launch_cache4_expand(x, st)) return e;
+        PromptAttn p;
+        p.q = q;
+        p.k = x.k;
+        p.v = x.v;
+        p.q_seq = s[0];
+        p.q_row = s[1];
+        p.q_head = s[2];
+        p.past_len = x.past_out;
+        p.sinks = sinks;
+        p.out = out;
+        p.half = x.half;
+        p.batch = a.c.batch;
+        p.seq = seq;
+        p.heads = heads;
+        p.kv_heads = a.c.kv_heads;
+        p.dim = a.c.dim;
+        p.span = plan.span;
+        p.max_seq = a.c.max_seq;
+        p.window = window;
+        p.scale = scale;
+        return launch_prompt_attn(p, st);
+    }
     a.q = q;
     a.qb = s[0];
     a.qs = s[1];
     a.qh = s[2];
     a.dtype = dtype;
-    a.wide = (((uintptr_t)q | (uintptr_t)((s[0] | s[1] | s[2]) * size)) & 15) == 0;
     a.out = out;
     a.part = static_cast<float*>(workspace);
     a.sinks = sinks;
-    a.past = Past{past_len, past};
     a.heads = heads;
     a.group = heads / a.c.kv_heads;
     a.seq = seq;
     a.rows = seq * a.group;
     a.window = window;
-    a.scale2 = scale * 1.4426950408889634f;
-    const Attend4Plan plan = attend4_plan(a.c, a.rows, attend4_reach(a.c, seq, past_len ? longest : past, window));
-    if (plan.part_bytes > workspace_bytes) return ROTOR_B200_ERR_WORKSPACE;
     a.splits = plan.splits;
-    const cudaStream_t st = as_stream(stream);
+    a.scale2 = scale * 1.4426950408889634f;
     switch (a.c.dim / C4_GROUP) {
         case 1: return attend4_pick<1>(a, plan, st);
         case 2: return attend4_pick<2>(a, plan, st);

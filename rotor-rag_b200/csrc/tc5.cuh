@@ -196,6 +196,11 @@ __host__ __device__ constexpr uint32_t t5_idesc_bf16(int m, int n, bool b_mn = f
            ((uint32_t)(m >> 4) << 24);
 }
 
+// The same with float16 operands.
+__host__ __device__ constexpr uint32_t t5_idesc_f16(int m, int n, bool b_mn = false) {
+    return t5_idesc_bf16(m, n, b_mn) & ~((1u << 7) | (1u << 10));
+}
+
 __device__ __forceinline__ void t5_mma_ss(uint32_t d_tmem, uint64_t da, uint64_t db, uint32_t idesc, uint32_t accumulate) {
     asm volatile(
         "{\n\t"

@@ -188,7 +188,7 @@ _SIGNATURES.update({
     "rotor_b200_reorder_states": (_i, [C.POINTER(State), _i, _p, _i, _i, _p]),
     "rotor_b200_cache4_append": (_i, [_c4p, _p, _p, _i, _sdp, _sdp, _i, _i, _p, _p]),
     "rotor_b200_cache4_read": (_i, [_c4p, _i, _i, _p, _p, _i, _p]),
-    "rotor_b200_cache4_attend_workspace_bytes": (_sz, [_c4p, _i, _i, _i, _i]),
+    "rotor_b200_cache4_attend_workspace_bytes": (_sz, [_c4p, _i, _i, _i, _i, _i]),
     "rotor_b200_cache4_attend": (_i, [_c4p, _p, _i, _sdp, _i, _i, _i, _p, _i, _f, _i, _p, _p, _p, _sz, _p]),
 })
 

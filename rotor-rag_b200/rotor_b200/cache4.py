@@ -106,7 +106,7 @@ class Cache4:
         Query head h reads KV head h // (heads // kv_heads).  ``scale`` of the scores: 1 / sqrt(dim) unless given.  ``window`` > 0: a
         query sees that many positions, its own included.  ``sinks`` float32 [heads]: exp(sink) joins the softmax's denominator.
         ``longest``: with a tensor of lengths, the most that a sequence holds, by which the work is divided (the cache's size unless
-        given; a wrong bound costs time, not results).  A query that sees no position gives zeros."""
+        given); longer lengths are taken as it.  A query that sees no position gives zeros."""
         torch = abi.require_cuda()
         heads = q.shape[2] if q.dim() == 4 else 0
         strides = self._rows("q", q, heads)
@@ -124,7 +124,7 @@ class Cache4:
         if seq == 0:
             return out
         bound = number if lengths is None else self.max_seq if longest is None else min(max(int(longest), 0), self.max_seq)
-        need = lib.rotor_b200_cache4_attend_workspace_bytes(self._ref, heads, seq, bound, window)
+        need = lib.rotor_b200_cache4_attend_workspace_bytes(self._ref, code, heads, seq, bound, window)
         if need == 0:
             raise RotorB200Error(f"{seq} queries of {heads} heads are beyond the attention's sizes")
         workspace = torch.empty(need, dtype=torch.uint8, device=q.device)

@@ -30,7 +30,7 @@ def test_descriptions_of_a_cache(kw, status):
     assert lib.rotor_b200_cache4_append(cache(**kw), A, A, 0, strides(), strides(), 1, 0, None, None) == status
     assert lib.rotor_b200_cache4_read(cache(**kw), 0, 1, A, A, 0, None) == status
     assert lib.rotor_b200_cache4_attend(cache(**kw), A, 0, strides(), 4, 1, 0, None, 0, 1.0, 0, None, A, A, 1 << 30, None) == status
-    assert lib.rotor_b200_cache4_attend_workspace_bytes(cache(**kw), 4, 1, 0, 0) == 0
+    assert lib.rotor_b200_cache4_attend_workspace_bytes(cache(**kw), 0, 4, 1, 0, 0) == 0
 
 
 def test_calls_on_a_cache():
@@ -48,9 +48,9 @@ def test_calls_on_a_cache():
     for kw in ({"q": None}, {"dtype": 7}, {"s": None}, {"s": strides(1, -1, 1)}, {"heads": 3}, {"heads": 0}, {"seq": 0}, {"seq": 33}, {"past": 32},
                {"past": -1}, {"longest": -1}, {"window": -1}, {"out": None}, {"out": A + 4}, {"ws": None}, {"ws": A + 8}, {"q": A + 1}):
         assert attend(**kw) == ARG, kw
-    need = lib.rotor_b200_cache4_attend_workspace_bytes(c, 4, 1, 5, 0)
+    need = lib.rotor_b200_cache4_attend_workspace_bytes(c, 0, 4, 1, 5, 0)
     assert need > 0 and attend(past=5, size=need - 1) == WORKSPACE
-    assert attend(heads=65536) == SHAPE and lib.rotor_b200_cache4_attend_workspace_bytes(c, 65536, 1, 5, 0) == 0
+    assert attend(heads=65536) == SHAPE and lib.rotor_b200_cache4_attend_workspace_bytes(c, 0, 65536, 1, 5, 0) == 0
 
 
 def test_selections():

@@ -6,6 +6,8 @@ and one more to the type asked for.  Attention is off by
  * the rounding of the weights: float16 (2^-11 at most, with the ratio to the sum of weights that are not rounded) of the weighted sums
    of |v| and of s code for 16-bit types, two terms (2^-21) for float32.  (s code, because a value is m + s code and the rounded weight
    p s multiplies the code alone: where m and s code cancel, p s code (1 + e) + p m = p v + e p s code.);
+ * 16-bit calls of 192 and more query rows a KV head: keys, values and weights are rounded to the type, h = finfo(type).eps / 2 each, which
+   is h of the weighted sum of |v| for the weights and for the values, and h of |q| |k| for a score, twice with the ratio to the sum;
  * scores: products accumulated in float32 over at most 256 columns and 8 groups, each addition off by 2^-23 of the sum of |q| |k|:
    fewer than 64 of them, so 2^-17 of it, which is the relative error of a weight, twice with the ratio to the sum."""
 import numpy as np
@@ -42,10 +44,13 @@ def held(x):
     return O.held(host(x)).transpose(0, 2, 1, 3)
 
 
-def check_attention(torch, got, want, size, reach, dtype):
+def check_attention(torch, got, want, size, reach, dtype, kv):
     half = torch.finfo(getattr(torch, dtype)).eps / 2
     weight = 2.0 ** -21 if dtype == "float32" else 2.0 ** -11
-    bound = half * np.abs(want) + size * (weight + 2.0 ** -16 * (reach[..., None] + 1)) + 1e-30
+    score = 2.0 ** -16
+    if dtype != "float32" and want.shape[1] * want.shape[2] // kv >= 192 and want.shape[3] <= 128:
+        weight, score = 2 * half, 2 * half + score
+    bound = half * np.abs(want) + size * (weight + score * (reach[..., None] + 1)) + 1e-30
     err = np.abs(host(got) - want)
     assert np.all(err <= bound), float((err / bound).max())
 
@@ -68,7 +73,7 @@ def attend_case(torch, seed, batch, seq, heads, kv, dim, past, window=0, sinks=F
     assert got.shape == q.shape and got.dtype == q.dtype
     want = O.attend(host(q), held(k), held(v), past, dim ** -0.5 if scale is None else scale, window, None if s is None else host(s),
                     O.coded(host(v)).transpose(0, 2, 1, 3))
-    check_attention(torch, got, *want, dtype)
+    check_attention(torch, got, *want, dtype, kv)
 
 
 @pytest.mark.parametrize("dtype", TYPES)
@@ -194,10 +199,23 @@ def test_windows_and_sinks(torch, window, dtype):
     attend_case(torch, window, 2, 1, 8, 2, 128, [0, 200], window=window, dtype=dtype, lengths=200)
 
 
-@pytest.mark.parametrize("lengths", [None, 1, 700, 10 ** 6])
-def test_unequal_lengths_and_any_bound(torch, lengths):
+@pytest.mark.parametrize("lengths", [None, 699, 700, 10 ** 6])
+def test_unequal_lengths_and_bounds(torch, lengths):
     attend_case(torch, 7, 6, 1, 8, 2, 64, [0, 1, 63, 64, 500, 699], dtype="bfloat16", lengths=lengths)
     attend_case(torch, 8, 3, 4, 8, 2, 64, [0, 17, 612], dtype="float32", lengths=lengths)
+
+
+@pytest.mark.parametrize("seq", [1, 64])
+@pytest.mark.parametrize("dtype", TYPES)
+def test_lengths_above_the_bound_are_taken_as_it(torch, seq, dtype):
+    from rotor_b200.cache4 import Cache4
+    rng = np.random.default_rng(18)
+    cache = Cache4(2, 1, 200, 64)
+    k = make(torch, rng, (2, 200, 1, 64), dtype)
+    cache.append(k, k, 0)
+    q = make(torch, rng, (2, seq, 2, 64), dtype)
+    past = lambda *n: torch.tensor(n, dtype=torch.int32, device="cuda")
+    assert torch.equal(cache.attend(q, past(120, 60), longest=100), cache.attend(q, past(100, 60), longest=100))
 
 
 @pytest.mark.parametrize("dtype", TYPES)
@@ -267,7 +285,8 @@ def test_query_rows_of_any_strides(torch):
             odd = make(torch, rng, (2, seq, 6, 65), dtype)[..., 1:]
             turned = make(torch, rng, (2, 6, seq, 64), dtype).transpose(1, 2)
             for q in (row[:, :, 3:], odd, turned, row[:1, :, :6].expand(2, seq, 6, 64)):
-                assert torch.equal(cache.attend(q, 5), cache.attend(q.contiguous(), 5))
+                want = O.attend(host(q), held(k), held(k), [5, 5], 0.125, 0, None, O.coded(host(k)).transpose(0, 2, 1, 3))
+                check_attention(torch, cache.attend(q, 5), *want, dtype, 2)
 
 
 def test_empty_calls(torch):
@@ -291,14 +310,14 @@ def test_a_query_beyond_the_cache_with_a_window_gives_zeros(torch):
     assert (cache.attend(torch.ones((1, 1, 2, 64), device="cuda"), past, window=2) == 1).all()
 
 
-@pytest.mark.parametrize("seq", [1, 24])
-def test_captured_steps_follow_the_lengths(torch, seq):
+@pytest.mark.parametrize("seq,dtype", [(1, "float32"), (1, "bfloat16"), (24, "float32"), (24, "bfloat16"), (24, "float16")])
+def test_captured_steps_follow_the_lengths(torch, seq, dtype):
     """Append and attend captured once on a side stream and replayed with other inputs and lengths."""
     from rotor_b200.cache4 import Cache4
     rng = np.random.default_rng(16)
     batch, kv, dim = 2, 2, 64
     cache, plain = Cache4(batch, kv, 128, dim), Cache4(batch, kv, 128, dim)
-    k, v, q = (torch.zeros((batch, seq, n, dim), device="cuda") for n in (kv, kv, 8))
+    k, v, q = (torch.zeros((batch, seq, n, dim), device="cuda", dtype=getattr(torch, dtype)) for n in (kv, kv, 8))
     past = torch.zeros(batch, dtype=torch.int32, device="cuda")
     stream = torch.cuda.Stream()
     stream.wait_stream(torch.cuda.current_stream())
@@ -313,7 +332,7 @@ def test_captured_steps_follow_the_lengths(torch, seq):
     lengths = np.array([0, 40])
     for _ in range(3):
         for t in (k, v, q):
-            t.copy_(make(torch, rng, tuple(t.shape), "float32"))
+            t.copy_(make(torch, rng, tuple(t.shape), dtype))
         past.copy_(torch.from_numpy(lengths.astype(np.int32)))
         graph.replay()
         plain.append(k, v, past)
