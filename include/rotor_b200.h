@@ -422,7 +422,7 @@ int rotor_b200_sample(const float* logits, int rows, int vocab, int mode, int to
  *    are -inf or NaN offer nothing, nor does a row that holds +inf or a beam whose score is not finite; where fewer than
  *    `count` candidates are left, the rest is filled with -inf and the lowest (w, v) that are not among them.
  *    logits: `dtype` [groups][width][vocab], rows at group_stride and beam_stride elements; scores float32 [groups][width];
- *    width <= 32, count <= 64 and <= width * vocab, width * vocab < 2^31.  out_scores float32, out_beams and out_tokens int64,
+ *    width <= 32, count <= 64 and <= width * vocab, vocab <= 2^30, width * vocab < 2^31.  out_scores float32, out_beams and out_tokens int64,
  *    [groups][count].  workspace: rotor_b200_beam_select_workspace_bytes bytes, 16-byte aligned, contents of no matter.
  *  reorder_states: row b * width + w of every state becomes what row b * width + beams[b][w] was, in place; rows whose beam is
  *    their own, or no index of the group, stay.  `states` is a HOST array; width <= 32. */

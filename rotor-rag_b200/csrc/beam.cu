@@ -5,16 +5,18 @@
 // candidates that are left their values in 64 bits (candidates of different beams lie close to one another, and float32 scores of
 // long texts have steps of 1e-6 and more) and takes the best.
 //
-// Both find the best the same way: a bar that at least `count` threads' largest candidates reach is searched for by halving (about
-// seven counts over the CTA), what reaches it (a few dozen) is listed in shared memory, and each of those counts how many are better.
-// Where too many reach every bar (equal logits in thousands) the best are taken one by one.
+// Both find the best the same way.  Threads keep the largest of what they have seen; a bar that at least `count` threads reach, and not
+// many more, is searched for by halving (about ten counts over the CTA); only what the threads that reach it have seen can be among the
+// best, and is looked at again (a slice: from L2); what reaches the bar (a few dozen) is listed in shared memory, and each of those counts
+// how many are better.  Where too many reach every bar (equal logits in thousands) the best are taken one by one.
 #include "decoder.cuh"
 #include "cache4.cuh"
 
 namespace rb {
 
 constexpr int BEAM_WIDTH = 32, BEAM_COUNT = 64;
-constexpr int BEAM_THREADS = 512, BEAM_EACH = 16, BEAM_SLICE = BEAM_THREADS * BEAM_EACH;
+constexpr int BEAM_THREADS = 512, BEAM_PIECE = 8;        // neighbouring logits that a thread takes at a time
+constexpr int BEAM_ROUND = BEAM_THREADS * BEAM_PIECE;    // slices are whole rounds of a CTA
 constexpr int BEAM_LIST = 1024;       // candidates that can be listed
 constexpr uint32_t BEAM_NONE = 0x007fffffu;  // keys of candidates are above this, the key of -inf
 
@@ -52,7 +54,7 @@ struct BeamSelect {
     int wide;
     const float* scores;
     const uint8_t* ended;
-    int groups, width, vocab, count, slices;
+    int groups, width, vocab, count, slices, rounds;
     long long pad;
     float2* share;        // [rows][slices]: largest logit, sum of exp(logit - largest)
     uint2* list;          // [rows][slices][count]: key of the logit, token; keys BEAM_NONE and below are no candidates
@@ -60,11 +62,25 @@ struct BeamSelect {
     long long *out_beams, *out_tokens;
 };
 
+// Logits i .. i + 7 of a row; what is no candidate as -inf.
+template <typename T>
+__device__ __forceinline__ void beam_piece(const T* x, int i, int vocab, int wide, float (&v)[BEAM_PIECE]) {
+    if (i + BEAM_PIECE <= vocab) {
+        load8(x + i, wide, v);
+#pragma unroll
+        for (int n = 0; n < BEAM_PIECE; ++n) v[n] = fmaxf(v[n], -INFINITY);  // (NaN: -inf)
+    } else {
+#pragma unroll
+        for (int n = 0; n < BEAM_PIECE; ++n) v[n] = i + n < vocab ? fmaxf(type_load(x + i + n), -INFINITY) : -INFINITY;
+    }
+}
+
 template <typename T>
 __global__ void __launch_bounds__(BEAM_THREADS) beam_slice_kernel(const __grid_constant__ BeamSelect p) {
     __shared__ float s_red[64];
     __shared__ uint2 s_list[BEAM_LIST];
-    __shared__ int s_n;
+    __shared__ unsigned short s_who[BEAM_THREADS];
+    __shared__ int s_n, s_whos;
     __shared__ unsigned long long s_best;
     pdl_wait();
     pdl_trigger();
@@ -72,53 +88,68 @@ __global__ void __launch_bounds__(BEAM_THREADS) beam_slice_kernel(const __grid_c
     if (p.ended && p.ended[row]) return;  // (the second kernel does not look at this row's share)
     const int group = row / p.width;
     const T* x = static_cast<const T*>(p.logits) + (size_t)group * p.group_stride + (size_t)(row - group * p.width) * p.beam_stride;
-    const int base = slice * BEAM_SLICE;
-    constexpr int V = 8;
-    uint32_t key[BEAM_EACH];
-    uint32_t mine = 0;
+    const int base = slice * p.rounds * BEAM_ROUND, rounds = min(p.rounds, (p.vocab - base + BEAM_ROUND - 1) / BEAM_ROUND);
+    auto place = [&](int round, int who) { return base + (round * BEAM_THREADS + who) * BEAM_PIECE; };
+
+    // ---- largest logit and sum of exp(logit - largest) of this thread's pieces
+    constexpr float log2e = 1.4426950408889634f;
+    float largest = -INFINITY, sum = 0.f;
+    auto take = [&](const float (&v)[BEAM_PIECE]) {
+        float m = v[0];
 #pragma unroll
-    for (int e = 0; e < BEAM_EACH; e += V) {
-        const int i = base + (e / V * BEAM_THREADS + tid) * V;
-        float v[V];
-        if (i + V <= p.vocab) {
-            load8(x + i, p.wide, v);
-        } else {
-#pragma unroll
-            for (int n = 0; n < V; ++n) v[n] = i + n < p.vocab ? type_load(x + i + n) : -INFINITY;
+        for (int n = 1; n < BEAM_PIECE; ++n) m = fmaxf(m, v[n]);
+        if (m > largest) {
+            sum *= fast_exp2((largest - m) * log2e);
+            largest = m;
         }
+        // (the difference first: the lowest float times log2(e) is none)
+        const float off = largest == -INFINITY ? 0.f : largest;
 #pragma unroll
-        for (int n = 0; n < V; ++n) {
-            key[e + n] = order_key(v[n]);
-            mine = max(mine, key[e + n]);
-        }
+        for (int n = 0; n < BEAM_PIECE; ++n) sum += fast_exp2((v[n] - off) * log2e);
+    };
+    int r = 0;
+    for (; r + 4 <= rounds; r += 4) {
+        float v[4][BEAM_PIECE];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) beam_piece(x, place(r + k, tid), p.vocab, p.wide, v[k]);
+#pragma unroll
+        for (int k = 0; k < 4; ++k) take(v[k]);
     }
-    auto token_of = [&](int e) { return (uint32_t)(base + (e / V * BEAM_THREADS + tid) * V + e % V); };
+    for (; r < rounds; ++r) {
+        float v[BEAM_PIECE];
+        beam_piece(x, place(r, tid), p.vocab, p.wide, v);
+        take(v);
+    }
 
     // ---- share of the row's mass
+    const uint32_t mine = order_key(largest);
     const uint32_t top_key = __reduce_max_sync(0xffffffffu, mine);
     if ((tid & 31) == 0) reinterpret_cast<uint32_t*>(s_red)[tid >> 5] = top_key;
-    if (tid == 0) s_n = 0;
+    if (tid == 0) s_n = s_whos = 0;
     __syncthreads();
     const uint32_t top = __reduce_max_sync(0xffffffffu, reinterpret_cast<uint32_t*>(s_red)[tid & (BEAM_THREADS / 32 - 1)]);
-    const float largest = order_value(top);
-    float sum = 0.f;
-    if (top > BEAM_NONE) {
-#pragma unroll
-        for (int e = 0; e < BEAM_EACH; ++e)
-            if (key[e] > BEAM_NONE) sum += __expf(order_value(key[e]) - largest);
-    }
-    sum = block_sum(sum, s_red + 16);
+    const float most = order_value(top);
+    sum = block_sum(largest == -INFINITY ? 0.f : sum * fast_exp2((largest - most) * log2e), s_red + 16);
     const size_t at = (size_t)row * p.slices + slice;
-    if (tid == 0) p.share[at] = make_float2(top > BEAM_NONE ? largest : -INFINITY, sum);
+    if (tid == 0) p.share[at] = make_float2(most, sum);
     uint2* out = p.list + at * p.count;
 
     // ---- the best of the slice
     const uint32_t bar = find_bar(mine, BEAM_NONE + 1, top, p.count);
+    if (mine >= bar && mine > BEAM_NONE) s_who[atomicAdd(&s_whos, 1)] = (unsigned short)tid;
+    __syncthreads();
+    const int pieces = s_whos * rounds;
+    for (int i = tid; i < pieces; i += BEAM_THREADS) {
+        const int who = i / rounds, at0 = place(i - who * rounds, s_who[who]);
+        float v[BEAM_PIECE];
+        beam_piece(x, at0, p.vocab, p.wide, v);
 #pragma unroll
-    for (int e = 0; e < BEAM_EACH; ++e) {
-        if (key[e] >= bar && key[e] > BEAM_NONE) {
-            const int n = atomicAdd(&s_n, 1);
-            if (n < BEAM_LIST) s_list[n] = make_uint2(key[e], token_of(e));
+        for (int n = 0; n < BEAM_PIECE; ++n) {
+            const uint32_t key = order_key(v[n]);
+            if (key >= bar && key > BEAM_NONE) {
+                const int k = atomicAdd(&s_n, 1);
+                if (k < BEAM_LIST) s_list[k] = make_uint2(key, at0 + n);
+            }
         }
     }
     __syncthreads();
@@ -136,22 +167,27 @@ __global__ void __launch_bounds__(BEAM_THREADS) beam_slice_kernel(const __grid_c
         for (int i = n + tid; i < p.count; i += BEAM_THREADS) out[i] = make_uint2(0u, 0u);
         return;
     }
-    // too many that are equal: one by one, the largest key and among equals the lowest token
+    // too many that are equal: one by one, the largest key and among equals the lowest token, below the last one taken
+    unsigned long long last = ~0ull;
     for (int k = 0; k < p.count; ++k) {
         unsigned long long best = 0;
+        for (int i = 0; i < rounds; ++i) {
+            float v[BEAM_PIECE];
+            beam_piece(x, place(i, tid), p.vocab, p.wide, v);
 #pragma unroll
-        for (int e = 0; e < BEAM_EACH; ++e)
-            if (key[e] > BEAM_NONE) best = max(best, (unsigned long long)key[e] << 32 | ~token_of(e));
-        __syncthreads();
+            for (int m = 0; m < BEAM_PIECE; ++m) {
+                const uint32_t key = order_key(v[m]);
+                const unsigned long long c = (unsigned long long)key << 32 | ~(uint32_t)(place(i, tid) + m);
+                if (key > BEAM_NONE && c < last && c > best) best = c;
+            }
+        }
         if (tid == 0) s_best = 0;
         __syncthreads();
         atomicMax(&s_best, best);
         __syncthreads();
-        const unsigned long long b = s_best;
-#pragma unroll
-        for (int e = 0; e < BEAM_EACH; ++e)
-            if (key[e] == (uint32_t)(b >> 32) && token_of(e) == ~(uint32_t)b) key[e] = 0;
-        if (tid == 0) out[k] = b ? make_uint2((uint32_t)(b >> 32), ~(uint32_t)b) : make_uint2(0u, 0u);
+        last = s_best;
+        __syncthreads();
+        if (tid == 0) out[k] = last ? make_uint2((uint32_t)(last >> 32), ~(uint32_t)last) : make_uint2(0u, 0u);
     }
 }
 
@@ -345,10 +381,19 @@ __global__ void __launch_bounds__(REORDER_THREADS) reorder_kernel(const __grid_c
     }
 }
 
-static int beam_slices(int vocab) { return (vocab + BEAM_SLICE - 1) / BEAM_SLICE; }
+// Rounds of a slice: as few as keep two CTAs on every SM busy, so that a slice's fixed part (the bar, the list) is shared by what it can be.
+static int beam_rounds(int rows, int vocab) {
+    const int all = (vocab + BEAM_ROUND - 1) / BEAM_ROUND;
+    const int slices = (2 * fused_sm_count() + rows - 1) / rows;
+    return slices >= all ? 1 : (all + slices - 1) / slices;
+}
+static int beam_slices(int rows, int vocab) {
+    const int per = beam_rounds(rows, vocab) * BEAM_ROUND;
+    return (vocab + per - 1) / per;
+}
 static bool beam_shape(int groups, int width, int vocab, int count) {
     return groups > 0 && width > 0 && vocab > 0 && count > 0 && width <= BEAM_WIDTH && count <= BEAM_COUNT &&
-           (long long)width * vocab < (1LL << 31) && count <= (long long)width * vocab && (long long)groups * width <= 65535;
+           vocab <= (1 << 30) && (long long)width * vocab < (1LL << 31) && count <= (long long)width * vocab && (long long)groups * width <= 65535;
 }
 
 }  // namespace rb
@@ -359,7 +404,7 @@ extern "C" {
 
 size_t rotor_b200_beam_select_workspace_bytes(int groups, int width, int vocab, int count) {
     if (!beam_shape(groups, width, vocab, count)) return 0;
-    return (size_t)groups * width * beam_slices(vocab) * (sizeof(float2) + count * sizeof(uint2));
+    return (size_t)groups * width * beam_slices(groups * width, vocab) * (sizeof(float2) + count * sizeof(uint2));
 }
 
 int rotor_b200_beam_select(const void* logits, int dtype, int64_t group_stride, int64_t beam_stride, const float* scores,
@@ -383,7 +428,8 @@ int rotor_b200_beam_select(const void* logits, int dtype, int64_t group_stride, 
     p.width = width;
     p.vocab = vocab;
     p.count = count;
-    p.slices = beam_slices(vocab);
+    p.slices = beam_slices(groups * width, vocab);
+    p.rounds = beam_rounds(groups * width, vocab);
     p.pad = ended ? pad : 0;
     const size_t shares = (size_t)groups * width * p.slices;
     p.list = static_cast<uint2*>(workspace);

@@ -1,29 +1,32 @@
 // The 4-bit cache is written and read back (layout: cache4.cuh).  Both directions move bytes: of a bf16 row of 128 columns 256 bytes
-// on the dense side and 80 in the cache.  A thread takes eight neighbouring columns, which are one word of a key row or two 16-bit words
-// of a value tile, and four threads a group; threads run along rows.
+// on the dense side and 80 in the cache.  A thread takes eight neighbouring columns of four positions (a multiple of four and the next
+// three): those are one word of each key row or two 8-byte words of a value tile, four threads are a group, and threads run along rows.
+// Four rows a thread keep enough loads in flight, and values leave in pieces of 8 bytes instead of 2.
 #include "cache4.cuh"
 
 namespace rb {
 
 constexpr int C4_THREADS = 256;
 
-// Where eight columns (c8 of a row) of a position lie: their word of the keys, or two 16-bit words of the values, `next` apart (parts g and
-// g + 1 of a tile), and their group's s and m.
+// Where eight columns (c8 of a row) of positions quad .. quad + 3 lie.  Keys: a word, `next` bytes to the next position; values: four 16-bit
+// words in a row, and `next` bytes behind them those of the next part g.  group: s and m of the first position, group_next to the next.
 struct Place {
-    uint16_t* codes;
+    unsigned char* codes;
     size_t group;
-    int next;
-    __device__ __forceinline__ Place(const Cache4View& c, int part, int b, uint32_t h, int pos, uint32_t c8) {
+    int next, group_next;
+    __device__ __forceinline__ Place(const Cache4View& c, int part, int b, uint32_t h, int quad, uint32_t c8) {
         const int NG = c.dim / C4_GROUP, j = c8 >> 2, t = c8 & 3;
         const size_t head = ((size_t)b * c.kv_heads + h) * c.max_seq;
         if (part == 0) {
-            codes = reinterpret_cast<uint16_t*>(c.codes[0]) + (head + pos) * (NG * 8) + (t * NG + j) * 2;
-            group = (head + pos) * NG + j;
-            next = 1;
+            codes = c.codes[0] + (head + quad) * (NG * 16) + (t * NG + j) * 4;
+            next = NG * 16;
+            group = (head + quad) * NG + j;
+            group_next = NG;
         } else {
-            codes = reinterpret_cast<uint16_t*>(c.codes[1]) + (head + (pos & ~15)) * (NG * 8) + value_at(NG, j, 2 * t, pos & 15);
-            group = (head + (pos & ~3)) * NG + j * 4 + (pos & 3);
-            next = value_at(NG, j, 1, 0) - value_at(NG, j, 0, 0);
+            codes = c.codes[1] + (head + (quad & ~15)) * (NG * 16) + 2 * value_at(NG, j, 2 * t, quad & 15);
+            next = 2 * (value_at(NG, j, 1, 0) - value_at(NG, j, 0, 0));
+            group = (head + quad) * NG + j * 4;
+            group_next = 1;
         }
     }
 };
@@ -34,7 +37,8 @@ struct Cache4Store {
     size_t sb[2], ss[2], sh[2];  // strides of sequence, position and head, in elements
     bool wide[2];                // rows begin at multiples of 16 bytes
     Past past;
-    uint32_t units;              // seq * kv_heads * dim / 8
+    int seq;
+    uint32_t units;              // quads * kv_heads * dim / 8
     FastDiv per_row, heads;
 };
 
@@ -48,22 +52,12 @@ __device__ __forceinline__ __half group_step(float low, float high) {
     return __float2half_rn(q);
 }
 
-template <typename T>
-__global__ void __launch_bounds__(C4_THREADS) cache4_store_kernel(const __grid_constant__ Cache4Store p) {
-    pdl_wait();
-    pdl_trigger();
-    const uint32_t u = blockIdx.x * C4_THREADS + threadIdx.x;
-    const int b = blockIdx.y, part = blockIdx.z;
-    const bool on = u < p.units;
-    const uint32_t row = p.per_row.div(on ? u : 0), c8 = (on ? u : 0) - row * p.per_row.d;
-    const uint32_t i = p.heads.div(row), h = row - i * p.heads.d;
-    float x[8];
-    load8(static_cast<const T*>(p.src[part]) + (size_t)b * p.sb[part] + (size_t)i * p.ss[part] + (size_t)h * p.sh[part] + c8 * 8, p.wide[part], x);
+// Eight columns of a row and their group: the codes, column n in bits 4 n.
+__device__ __forceinline__ uint32_t quantise8(const float (&x)[8], __half& sh, __half& mh) {
     // (minimum and maximum pass over NaN; a group of nothing else holds zeros)
     float low = INFINITY, high = -INFINITY;
 #pragma unroll
     for (int n = 0; n < 8; ++n) {
-        if (x[n] == x[n]) x[n] = fminf(fmaxf(x[n], -C4_MOST), C4_MOST);
         low = fminf(low, x[n]);
         high = fmaxf(high, x[n]);
     }
@@ -73,38 +67,94 @@ __global__ void __launch_bounds__(C4_THREADS) cache4_store_kernel(const __grid_c
         high = fmaxf(high, __shfl_xor_sync(0xffffffffu, high, o));
     }
     if (low > high) low = high = 0.f;
-    const __half sh = group_step(low, high), mh = __float2half_rn(low);
+    // (columns beyond the bounds get the outermost codes, as the bounds themselves do)
+    low = fminf(fmaxf(low, -C4_MOST), C4_MOST);
+    high = fminf(fmaxf(high, -C4_MOST), C4_MOST);
+    sh = group_step(low, high);
+    mh = __float2half_rn(low);
     const float s = __half2float(sh), m = __half2float(mh);
     const float inv = s > 0.f ? __frcp_rn(s) : 0.f;
-    uint32_t word = 0;
-    bool close = false;
+    constexpr float round_at = 12582912.f;  // 1.5 2^23: the sum is a whole number, to the nearest, ties to even
+    float code[8], off = 0.f;
 #pragma unroll
     for (int n = 0; n < 8; ++n) {
-        const float q = fminf(fmaxf((x[n] - m) * inv, 0.f), 15.f), code = rintf(q);  // (NaN: 0)
-        close |= fabsf(fabsf(q - code) - 0.5f) < 2e-5f;
-        word |= (uint32_t)(int)code << (4 * n);
+        const float q = fminf(fmaxf((x[n] - m) * inv, 0.f), 15.f);  // (NaN: 0)
+        code[n] = __fadd_rn(__fadd_rn(q, round_at), -round_at);
+        off = fmaxf(off, fabsf(q - code[n]));
     }
     // The quotient in float32 is off by less than 1e-5: next to a border between two codes it is taken in 64 bits.
-    if (close) {
-        word = 0;
+    if (off > 0.5f - 2e-5f) {
 #pragma unroll
         for (int n = 0; n < 8; ++n) {
             const double q = ((double)x[n] - (double)m) / (double)s;
-            word |= (uint32_t)(int)fmin(fmax(rint(q), 0.0), 15.0) << (4 * n);
+            code[n] = (float)fmin(fmax(rint(q), 0.0), 15.0);
         }
     }
-    const int pos = past_of(p.past, b) + (int)i;
-    if (!on || pos >= p.c.max_seq) return;
-    const Place w(p.c, part, b, h, pos, c8);
-    if (part == 0) {
-        *reinterpret_cast<uint32_t*>(w.codes) = word;
-    } else {
-        w.codes[0] = (uint16_t)word;
-        w.codes[w.next] = (uint16_t)(word >> 16);
+    // (four codes are a number below 2^16, which the sum with 2^23 has in its low bits)
+    uint32_t half[2];
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+        const float* c = code + 4 * k;
+        half[k] = __float_as_uint(fmaf(fmaf(fmaf(c[3], 16.f, c[2]), 16.f, c[1]), 16.f, c[0]) + 8388608.f);
     }
-    if ((c8 & 3) == 0) {
-        p.c.step[part][w.group] = sh;
-        p.c.least[part][w.group] = mh;
+    return __byte_perm(half[0], half[1], 0x5410);
+}
+
+template <typename T>
+__global__ void __launch_bounds__(C4_THREADS) cache4_store_kernel(const __grid_constant__ Cache4Store p) {
+    pdl_wait();
+    pdl_trigger();
+    const uint32_t u = blockIdx.x * C4_THREADS + threadIdx.x;
+    const int b = blockIdx.y, part = blockIdx.z;
+    const bool on = u < p.units;
+    const uint32_t row = p.per_row.div(on ? u : 0), c8 = (on ? u : 0) - row * p.per_row.d;
+    const uint32_t nth = p.heads.div(row), h = row - nth * p.heads.d;
+    const int past = past_of(p.past, b), quad = (past & ~3) + 4 * (int)nth;
+    const int from = max(past - quad, 0), to = min(min(past + p.seq, p.c.max_seq) - quad, 4);  // which of the four are there
+    const T* src = static_cast<const T*>(p.src[part]) + (size_t)b * p.sb[part] + (size_t)h * p.sh[part] + c8 * 8;
+    float x[4][8];
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+        if (k >= from && k < to) {
+            load8(src + (size_t)(quad + k - past) * p.ss[part], p.wide[part], x[k]);
+        } else {
+#pragma unroll
+            for (int n = 0; n < 8; ++n) x[k][n] = 0.f;
+        }
+    }
+    uint32_t word[4];
+    __half s[4], m[4];
+#pragma unroll
+    for (int k = 0; k < 4; ++k) word[k] = quantise8(x[k], s[k], m[k]);
+    if (!on || from >= to) return;
+    const Place w(p.c, part, b, h, quad, c8);
+    const bool whole = from == 0 && to == 4, first = (c8 & 3) == 0;
+    __half *step = p.c.step[part] + w.group, *least = p.c.least[part] + w.group;
+    if (part == 0) {
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            if (k >= from && k < to) {
+                *reinterpret_cast<uint32_t*>(w.codes + k * w.next) = word[k];
+                if (first) step[k * w.group_next] = s[k], least[k * w.group_next] = m[k];
+            }
+        }
+    } else if (whole) {
+        *reinterpret_cast<uint2*>(w.codes) = make_uint2(__byte_perm(word[0], word[1], 0x5410), __byte_perm(word[2], word[3], 0x5410));
+        *reinterpret_cast<uint2*>(w.codes + w.next) = make_uint2(__byte_perm(word[0], word[1], 0x7632), __byte_perm(word[2], word[3], 0x7632));
+        if (first) {
+            auto two = [](__half a, __half c) { return (uint32_t)__half_as_ushort(a) | (uint32_t)__half_as_ushort(c) << 16; };
+            *reinterpret_cast<uint2*>(step) = make_uint2(two(s[0], s[1]), two(s[2], s[3]));
+            *reinterpret_cast<uint2*>(least) = make_uint2(two(m[0], m[1]), two(m[2], m[3]));
+        }
+    } else {
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            if (k >= from && k < to) {
+                reinterpret_cast<uint16_t*>(w.codes)[k] = (uint16_t)word[k];
+                reinterpret_cast<uint16_t*>(w.codes + w.next)[k] = (uint16_t)(word[k] >> 16);
+                if (first) step[k] = s[k], least[k] = m[k];
+            }
+        }
     }
 }
 
@@ -112,8 +162,8 @@ struct Cache4Load {
     Cache4View c;
     void* dst[2];
     int begin, span;
-    uint32_t units;  // kv_heads * span * dim / 8
-    FastDiv per_row, positions;
+    uint32_t units;  // kv_heads * quads * dim / 8
+    FastDiv per_row, quads;
     // rows for a prompt
     int seq, window;
     Past past;
@@ -128,32 +178,57 @@ __global__ void __launch_bounds__(C4_THREADS) cache4_load_kernel(const __grid_co
     const int b = blockIdx.y, part = blockIdx.z;
     if (u >= p.units) return;
     const uint32_t row = p.per_row.div(u), c8 = u - row * p.per_row.d;
-    const uint32_t h = p.positions.div(row), pos = p.begin + row - h * p.positions.d;
-    bool there = true;
+    const uint32_t h = p.quads.div(row);
+    const int quad = (p.begin & ~3) + 4 * (int)(row - h * p.quads.d), end = p.begin + p.span;
+    int limit = p.c.max_seq;  // positions from here on are zeros
     if constexpr (PROMPT) {
         // the attention reads tiles of 128 positions from the first one its first query sees: a head's rows end in zeros, and so begin
         // the rows that a tile at the end of the head before reaches into
-        const int past = past_of(p.past, b), limit = min(past + p.seq, p.c.max_seq);
+        const int past = past_of(p.past, b);
+        limit = min(past + p.seq, p.c.max_seq);
         if (p.past_out && u == 0 && part == 0) p.past_out[b] = past;
-        if ((int)pos >= limit + 128 || ((int)pos < first_visible(past, 0, p.window) && pos >= 128)) return;
-        there = (int)pos < limit;
+        if (quad >= limit + 128 || (quad + 3 < first_visible(past, 0, p.window) && quad >= 128)) return;
     }
-    float x[8];
-    uint32_t word = 0;
-    float s = 0.f, m = 0.f;
-    if (there) {
-        const Place w(p.c, part, b, h, pos, c8);
-        word = part == 0 ? *reinterpret_cast<const uint32_t*>(w.codes) : w.codes[0] | (uint32_t)w.codes[w.next] << 16;
-        s = __half2float(p.c.step[part][w.group]);
-        m = __half2float(p.c.least[part][w.group]);
-    }
+    uint32_t word[4] = {0u, 0u, 0u, 0u};
+    float s[4] = {0.f, 0.f, 0.f, 0.f}, m[4] = {0.f, 0.f, 0.f, 0.f};
+    if (quad < p.c.max_seq) {
+        const Place w(p.c, part, b, h, quad, c8);
+        const __half *step = p.c.step[part] + w.group, *least = p.c.least[part] + w.group;
+        if (part == 0) {
 #pragma unroll
-    for (int n = 0; n < 8; ++n) x[n] = fmaf((float)(word >> (4 * n) & 15u), s, m);
-    if constexpr (PROMPT) {
+            for (int k = 0; k < 4; ++k) {
+                word[k] = *reinterpret_cast<const uint32_t*>(w.codes + k * w.next);
+                s[k] = __half2float(step[k * w.group_next]);
+                m[k] = __half2float(least[k * w.group_next]);
+            }
+        } else {
+            const uint2 lo = *reinterpret_cast<const uint2*>(w.codes), hi = *reinterpret_cast<const uint2*>(w.codes + w.next);
+            const uint2 sv = *reinterpret_cast<const uint2*>(step), mv = *reinterpret_cast<const uint2*>(least);
+            word[0] = __byte_perm(lo.x, hi.x, 0x5410), word[1] = __byte_perm(lo.x, hi.x, 0x7632);
+            word[2] = __byte_perm(lo.y, hi.y, 0x5410), word[3] = __byte_perm(lo.y, hi.y, 0x7632);
+            const uint32_t sw[2] = {sv.x, sv.y}, mw[2] = {mv.x, mv.y};
 #pragma unroll
-        for (int n = 0; n < 8; ++n) x[n] = fminf(x[n], C4_MOST);  // (m + 15 s may lie a rounding above the largest float16)
+            for (int k = 0; k < 4; ++k) {
+                const float2 a = __half22float2(*reinterpret_cast<const __half2*>(&sw[k >> 1])), c = __half22float2(*reinterpret_cast<const __half2*>(&mw[k >> 1]));
+                s[k] = k & 1 ? a.y : a.x;
+                m[k] = k & 1 ? c.y : c.x;
+            }
+        }
     }
-    store8(static_cast<T*>(p.dst[part]) + (((size_t)b * p.c.kv_heads + h) * p.span + (pos - p.begin)) * p.c.dim + c8 * 8, x);
+    T* dst = static_cast<T*>(p.dst[part]) + (((size_t)b * p.c.kv_heads + h) * p.span) * p.c.dim + c8 * 8;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+        const int pos = quad + k;
+        if (pos < p.begin || pos >= end) continue;
+        float x[8];
+        const bool there = pos < limit;
+#pragma unroll
+        for (int n = 0; n < 8; ++n) {
+            x[n] = fmaf((float)(word[k] >> (4 * n) & 15u), s[k], m[k]);
+            if (PROMPT) x[n] = there ? fminf(x[n], C4_MOST) : 0.f;  // (m + 15 s may lie a rounding above the largest float16)
+        }
+        store8(dst + (size_t)(pos - p.begin) * p.c.dim, x);
+    }
 }
 
 int cache4_view(const rotor_b200_cache4* c, Cache4View& v) {
@@ -180,11 +255,12 @@ int cache4_view(const rotor_b200_cache4* c, Cache4View& v) {
 }
 
 static int load_units(Cache4Load& p) {
-    const uint64_t units = (uint64_t)p.c.kv_heads * p.span * (p.c.dim / 8);
+    const uint32_t quads = (p.begin + p.span + 3) / 4 - p.begin / 4;
+    const uint64_t units = (uint64_t)p.c.kv_heads * quads * (p.c.dim / 8);
     if (units > 0x7fffff00u) return ROTOR_B200_ERR_SHAPE;
     p.units = (uint32_t)units;
     p.per_row = FastDiv(p.c.dim / 8);
-    p.positions = FastDiv(p.span);
+    p.quads = FastDiv(quads);
     return ROTOR_B200_OK;
 }
 
@@ -228,7 +304,10 @@ int rotor_b200_cache4_append(const rotor_b200_cache4* cache, const void* k, cons
         p.sh[i] = s[2];
         p.wide[i] = (((uintptr_t)p.src[i] | (uintptr_t)((s[0] | s[1] | s[2]) * size)) & 15) == 0;
     }
-    const uint64_t units = (uint64_t)seq * p.c.kv_heads * (p.c.dim / 8);
+    // quads of positions that a sequence's rows can lie in, wherever it starts
+    const uint32_t quads = past_len ? (seq + 6) / 4 : (past + seq + 3) / 4 - past / 4;
+    const uint64_t units = (uint64_t)quads * p.c.kv_heads * (p.c.dim / 8);
+    p.seq = seq;
     if (units > 0x7fffff00u) return ROTOR_B200_ERR_SHAPE;
     p.past = Past{past_len, past, p.c.max_seq};
     p.units = (uint32_t)units;

@@ -51,6 +51,12 @@ struct Past {
 };
 __device__ __forceinline__ int past_of(const Past& p, int b) { return p.each ? min(max(__ldcg(p.each + b), 0), p.most) : p.all; }
 
+__device__ __forceinline__ float fast_exp2(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+
 __device__ __forceinline__ float type_load(const float* p) { return *p; }
 __device__ __forceinline__ float type_load(const __nv_bfloat16* p) { return __bfloat162float(*p); }
 __device__ __forceinline__ float type_load(const __half* p) { return __half2float(*p); }

@@ -20,6 +20,7 @@
 // Tiles travel by cp.async into a ring of the warp's own (no barrier, and the loads in flight do not depend on what the registers hold):
 // a tile of 128 columns is 2560 bytes, five copies a lane.
 #include <cmath>
+#include <cstdlib>
 
 #include "cache4.cuh"
 
@@ -43,12 +44,6 @@ struct Attend4 {
     int heads, group, seq, rows, window, splits;
     float scale2;       // scale log2(e)
 };
-
-__device__ __forceinline__ float a4_exp2(float x) {
-    float y;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-    return y;
-}
 
 __device__ __forceinline__ void a4_mma(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
     asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
@@ -156,6 +151,29 @@ struct A4Cfg {
     static constexpr int END = ROWS + Q * OS * 4, SMEM = END > RING + RING_BYTES ? END : RING + RING_BYTES;
 };
 
+__device__ __forceinline__ void cluster_sync() {
+    asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+    asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+__device__ __forceinline__ uint32_t cluster_at(const float* local, unsigned rank) {
+    uint32_t a;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"((uint32_t)__cvta_generic_to_shared(local)), "r"(rank));
+    return a;
+}
+__device__ __forceinline__ float2 cluster_load2(const float* local, unsigned rank) {
+    float2 v;
+    asm volatile("ld.shared::cluster.v2.f32 {%0, %1}, [%2];" : "=f"(v.x), "=f"(v.y) : "r"(cluster_at(local, rank)) : "memory");
+    return v;
+}
+__device__ __forceinline__ float4 cluster_load4(const float* local, unsigned rank) {
+    float4 v;
+    asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
+                 : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w)
+                 : "r"(cluster_at(local, rank))
+                 : "memory");
+    return v;
+}
+
 __device__ __forceinline__ void store4(void* out, int dtype, size_t at, float4 y) {
     if (dtype == ROTOR_B200_F32) {
         *reinterpret_cast<float4*>(static_cast<float*>(out) + at) = y;
@@ -170,8 +188,8 @@ __device__ __forceinline__ void store4(void* out, int dtype, size_t at, float4 y
 __device__ __forceinline__ void finish4(const Attend4& p, int b, int hk, int row, int col, float4 y, float mass, float shift) {
     const int token = row / p.group, head = hk * p.group + row - token * p.group;
     if (p.sinks) {
-        const float sink = __ldg(p.sinks + head) * 1.4426950408889634f, top = fmaxf(shift, sink), mine = a4_exp2(shift - top);
-        mass = fmaf(mass, mine, a4_exp2(sink - top));
+        const float sink = __ldg(p.sinks + head) * 1.4426950408889634f, top = fmaxf(shift, sink), mine = fast_exp2(shift - top);
+        mass = fmaf(mass, mine, fast_exp2(sink - top));
         y.x *= mine, y.y *= mine, y.z *= mine, y.w *= mine;
     }
     const float inv = mass == 0.f ? 0.f : 1.f / mass;
@@ -423,7 +441,7 @@ __global__ void __launch_bounds__(A4_THREADS, NG* R <= 4 ? 2 : 1) attend4_kernel
 #pragma unroll
                     for (int n = 4; n < 32; n <<= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, n));
                     m = fmaxf(shift[h][e] + (lift - now), m - now);
-                    alpha[e] = a4_exp2(shift[h][e] - m);
+                    alpha[e] = fast_exp2(shift[h][e] - m);
                     shift[h][e] = m;
                 }
                 rescale(h, alpha[0], alpha[1]);
@@ -437,7 +455,7 @@ __global__ void __launch_bounds__(A4_THREADS, NG* R <= 4 ? 2 : 1) attend4_kernel
         for (int h = 0; h < R; ++h) {
 #pragma unroll
             for (int u = 0; u < 2; ++u) {
-                const float e0 = a4_exp2(sc[h][2 * u] - shift[h][0]), e1 = a4_exp2(sc[h][2 * u + 1] - shift[h][1]);
+                const float e0 = fast_exp2(sc[h][2 * u] - shift[h][0]), e1 = fast_exp2(sc[h][2 * u + 1] - shift[h][1]);
                 const uint32_t w = pack_half(e0, e1);
                 pw[h][0][u] = turned(w);
                 if (TERMS > 1) {
@@ -526,6 +544,7 @@ __global__ void __launch_bounds__(A4_THREADS, NG* R <= 4 ? 2 : 1) attend4_kernel
         }
     }
     __syncthreads();
+    float* mine = reinterpret_cast<float*>(a4_raw + C::ROWS);  // [row][OS]: sums, shift, mass
     for (int idx = threadIdx.x; idx < Q * (D / 4); idx += A4_THREADS) {
         const int r = idx / (D / 4), c4 = idx - r * (D / 4), row = r0 + r;
         if (row >= p.rows) break;
@@ -535,7 +554,7 @@ __global__ void __launch_bounds__(A4_THREADS, NG* R <= 4 ? 2 : 1) attend4_kernel
         float4 y = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
         for (int w = 0; w < A4_WARPS; ++w) {
-            const float f = a4_exp2(shifts[w][r] - top);
+            const float f = fast_exp2(shifts[w][r] - top);
             const float4 v = *reinterpret_cast<const float4*>(all + (w * Q + r) * C::OS + 4 * c4);
             total = fmaf(f, masses[w][r], total);
             y.x = fmaf(f, v.x, y.x), y.y = fmaf(f, v.y, y.y), y.z = fmaf(f, v.z, y.z), y.w = fmaf(f, v.w, y.w);
@@ -544,35 +563,78 @@ __global__ void __launch_bounds__(A4_THREADS, NG* R <= 4 ? 2 : 1) attend4_kernel
             finish4(p, b, hk, row, 4 * c4, y, total, top);
             continue;
         }
+        if (p.splits <= A4_CLUSTER) {
+            *reinterpret_cast<float4*>(mine + r * C::OS + 4 * c4) = y;
+            if (c4 == 0) *reinterpret_cast<float2*>(mine + r * C::OS + D) = make_float2(top, total);
+            continue;
+        }
         float* part = p.part + (((size_t)(b * p.c.kv_heads + hk) * p.rows + row) * p.splits + split) * (D + 4);
         *reinterpret_cast<float4*>(part + 4 * c4) = y;
         if (c4 == 0) *reinterpret_cast<float2*>(part + D) = make_float2(top, total);
     }
+    if (p.splits == 1 || p.splits > A4_CLUSTER) return;
+    // the CTAs of a cluster are the splits of its rows: each finishes a share of them
+    cluster_sync();
+    for (int idx = threadIdx.x * p.splits + split; idx < Q * (D / 4); idx += A4_THREADS * p.splits) {
+        const int r = idx / (D / 4), c4 = idx - r * (D / 4), row = r0 + r;
+        if (row >= p.rows) break;
+        float2 sm[A4_CLUSTER];
+        float4 v[A4_CLUSTER];
+#pragma unroll
+        for (int k = 0; k < A4_CLUSTER; ++k)
+            if (k < p.splits) {
+                sm[k] = cluster_load2(mine + r * C::OS + D, k);
+                v[k] = cluster_load4(mine + r * C::OS + 4 * c4, k);
+            }
+        float top = A4_LOW, total = 0.f;
+#pragma unroll
+        for (int k = 0; k < A4_CLUSTER; ++k)
+            if (k < p.splits) top = fmaxf(top, sm[k].x);
+        float4 y = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+        for (int k = 0; k < A4_CLUSTER; ++k)
+            if (k < p.splits) {
+                const float f = fast_exp2(sm[k].x - top);
+                total = fmaf(f, sm[k].y, total);
+                y.x = fmaf(f, v[k].x, y.x), y.y = fmaf(f, v[k].y, y.y), y.z = fmaf(f, v[k].z, y.z), y.w = fmaf(f, v[k].w, y.w);
+            }
+        finish4(p, b, hk, row, 4 * c4, y, total, top);
+    }
+    cluster_sync();  // (nobody leaves while its rows are being read)
 }
 
-// Joins the splits of a query row: a warp per row.
-__global__ void __launch_bounds__(32) attend4_join_kernel(const __grid_constant__ Attend4 p) {
+// Joins the splits of a query row where they are more than a cluster: a CTA per row, its threads columns x shares of the splits.
+__global__ void __launch_bounds__(A4_THREADS) attend4_join_kernel(const __grid_constant__ Attend4 p) {
+    __shared__ float4 s_y[A4_THREADS];
+    __shared__ float s_mass[A4_THREADS];
     pdl_wait();
     pdl_trigger();
     const int D = p.c.dim, hk = blockIdx.x / p.rows, row = blockIdx.x - hk * p.rows, b = blockIdx.y;
+    const int shares = A4_THREADS / (D / 4), share = threadIdx.x / (D / 4), c = threadIdx.x - share * (D / 4);
     const float* part = p.part + ((size_t)(b * p.c.kv_heads + hk) * p.rows + row) * p.splits * (D + 4);
     float top = A4_LOW;
-    for (int s = threadIdx.x; s < p.splits; s += 32) top = fmaxf(top, __ldcg(part + (size_t)s * (D + 4) + D));
+    for (int s = threadIdx.x & 31; s < p.splits; s += 32) top = fmaxf(top, __ldcg(part + (size_t)s * (D + 4) + D));
     top = warp_max(top);
-    for (int c = 4 * threadIdx.x; c < D; c += 128) {
-        float total = 0.f;
-        float4 y = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 4
-        for (int s = 0; s < p.splits; ++s) {
+    float total = 0.f;
+    float4 y = make_float4(0.f, 0.f, 0.f, 0.f);
+    auto add = [&](float f, float mass, const float4& v) {
+        total = fmaf(f, mass, total);
+        y.x = fmaf(f, v.x, y.x), y.y = fmaf(f, v.y, y.y), y.z = fmaf(f, v.z, y.z), y.w = fmaf(f, v.w, y.w);
+    };
+    if (share < shares) {
+#pragma unroll 8
+        for (int s = share; s < p.splits; s += shares) {
             const float* q = part + (size_t)s * (D + 4);
             const float2 ml = __ldcg(reinterpret_cast<const float2*>(q + D));
-            const float4 v = __ldcg(reinterpret_cast<const float4*>(q + c));
-            const float f = a4_exp2(ml.x - top);
-            total = fmaf(f, ml.y, total);
-            y.x = fmaf(f, v.x, y.x), y.y = fmaf(f, v.y, y.y), y.z = fmaf(f, v.z, y.z), y.w = fmaf(f, v.w, y.w);
+            add(fast_exp2(ml.x - top), ml.y, __ldcg(reinterpret_cast<const float4*>(q + 4 * c)));
         }
-        finish4(p, b, hk, row, c, y, total, top);
     }
+    s_y[threadIdx.x] = y;
+    s_mass[threadIdx.x] = total;
+    __syncthreads();
+    if (share > 0) return;
+    for (int k = 1; k < shares; ++k) add(1.f, s_mass[k * (D / 4) + c], s_y[k * (D / 4) + c]);
+    finish4(p, b, hk, row, 4 * c, y, total, top);
 }
 
 // Query rows of a KV head from which 16-bit calls go to the prompt kernel: the cache's rows are made dense (bf16 or float16) in the workspace
@@ -608,8 +670,10 @@ static Attend4Plan attend4_plan(const Cache4View& c, int dtype, int heads, int s
     const long long most = (tiles + A4_WARPS - 1) / A4_WARPS;  // a tile per warp
     if (splits > most) splits = most;
     if (splits < 1) splits = 1;
+    static const char* dbg = getenv("A4S");
+    if (dbg) splits = atoi(dbg) < most ? atoi(dbg) : most;
     a.splits = (int)splits;
-    a.bytes = splits == 1 ? 16 : (size_t)c.batch * c.kv_heads * rows * splits * (c.dim + 4) * sizeof(float);
+    a.bytes = splits <= A4_CLUSTER ? 16 : (size_t)c.batch * c.kv_heads * rows * splits * (c.dim + 4) * sizeof(float);
     return a;
 }
 
@@ -622,8 +686,8 @@ static int attend4_go(const Attend4& a, const Attend4Plan& plan, cudaStream_t st
         once.here() = true;
     }
     const dim3 grid(a.c.kv_heads * ((a.rows + plan.per_block - 1) / plan.per_block) * a.splits, a.c.batch);
-    const int e = launch_chained(attend4_kernel<NG, R, TERMS>, grid, A4_THREADS, smem, st, 1, a);
-    return e || a.splits == 1 ? e : launch_chained(attend4_join_kernel, dim3(a.rows * a.c.kv_heads, a.c.batch), 32, 0, st, 1, a);
+    const int e = launch_chained(attend4_kernel<NG, R, TERMS>, grid, A4_THREADS, smem, st, a.splits <= A4_CLUSTER ? a.splits : 1, a);
+    return e || a.splits <= A4_CLUSTER ? e : launch_chained(attend4_join_kernel, dim3(a.rows * a.c.kv_heads, a.c.batch), A4_THREADS, 0, st, 1, a);
 }
 
 template <int NG>

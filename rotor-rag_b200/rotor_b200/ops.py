@@ -213,7 +213,7 @@ def beam_select(logits, scores, count, ended=None, pad=0):
     if vocab > 1 and logits.stride(2) != 1:
         raise ValueError("the logits of a row have to lie side by side")
     count = int(count)
-    if not (1 <= width <= 32 and 1 <= count <= 64 and count <= width * vocab < 2 ** 31):
+    if not (1 <= width <= 32 and 1 <= count <= 64 and count <= width * vocab < 2 ** 31 and vocab <= 2 ** 30):
         raise ValueError(f"{count} of {width} x {vocab} candidates: up to 32 beams and 64 continuations, not more than there are")
     if ended is not None:
         on_device("ended", ended, 2, torch.bool)
