@@ -461,8 +461,10 @@ int rotor_b200_reorder_states(const rotor_b200_state* states, int n, const int64
  *    with window > 0 those with (own - j) < window.  Softmax of scale * q . k, whose denominator holds exp(sinks[head]) as well
  *    (sinks float32 [heads] or NULL); query head h reads KV head h / (heads / kv_heads).  out: `dtype` [batch][seq][heads][dim],
  *    16-byte aligned.  A query that sees no position gives zeros.  `longest`: with past_len, the most that a sequence holds, by which the
- *    work is divided; longer lengths are taken as it.  Without, not read but for the size of the workspace: 16-byte
- *    aligned, contents of no matter, rotor_b200_cache4_attend_workspace_bytes bytes with `longest` = past where past_len is NULL. */
+ *    work is divided; longer lengths are taken as it.  Without, not read.  workspace: 16-byte aligned, contents of no
+ *    matter, rotor_b200_cache4_attend_workspace_bytes bytes (given `longest` = past where past_len is NULL; 0: not supported); calls
+ *    that use none, steps of a few tokens over caches that are not long, take NULL, and the others return ERR_WORKSPACE before
+ *    anything is launched. */
 typedef struct rotor_b200_cache4 {
     int32_t batch, kv_heads, max_seq, dim;
     uint8_t *k_codes, *v_codes;

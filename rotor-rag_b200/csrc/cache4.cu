@@ -45,63 +45,96 @@ struct Cache4Store {
 // s of a group.  The definition rounds the quotient in 64 bits to float32 and then to float16.  float32 arithmetic gives the same
 // float16 unless its result is within a few of its own steps of a border between two float16 numbers.
 __device__ __forceinline__ __half group_step(float low, float high) {
-    const float q = __fdiv_rn(high - low, 15.f);
+    const float q = (high - low) * (1.f / 15.f);
     const int low_bits = __float_as_int(q) & 0x1fff;  // of a normal float16 these are cut off, and 0x1000 is the border
     if (high > low && (q < 6.2e-5f || (low_bits >= 0x1000 - 4 && low_bits <= 0x1000 + 4)))
         return __float2half_rn((float)(((double)high - (double)low) / 15.0));
     return __float2half_rn(q);
 }
 
-// Eight columns of a row and their group: the codes, column n in bits 4 n.
-__device__ __forceinline__ uint32_t quantise8(const float (&x)[8], __half& sh, __half& mh) {
-    // (minimum and maximum pass over NaN; a group of nothing else holds zeros)
-    float low = INFINITY, high = -INFINITY;
+__device__ __forceinline__ float fast_rcp(float x) {
+    float y;
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+
+// Smallest and largest of the groups of four rows x[k], of which each of four neighbouring threads holds eight columns: thread t of the
+// four gets those of row t.  (Rows are handed over by halves, so that every thread makes one row's s and m and not all four.)
+__device__ __forceinline__ void group_bounds(const float (&x)[4][8], int t, float& low, float& high) {
+    float lo[4], hi[4];
 #pragma unroll
-    for (int n = 0; n < 8; ++n) {
-        low = fminf(low, x[n]);
-        high = fmaxf(high, x[n]);
-    }
+    for (int k = 0; k < 4; ++k) {  // (minimum and maximum pass over NaN)
+        lo[k] = hi[k] = x[k][0];
 #pragma unroll
-    for (int o = 1; o < 4; o <<= 1) {
-        low = fminf(low, __shfl_xor_sync(0xffffffffu, low, o));
-        high = fmaxf(high, __shfl_xor_sync(0xffffffffu, high, o));
+        for (int n = 1; n < 8; ++n) {
+            lo[k] = fminf(lo[k], x[k][n]);
+            hi[k] = fmaxf(hi[k], x[k][n]);
+        }
     }
-    if (low > high) low = high = 0.f;
-    // (columns beyond the bounds get the outermost codes, as the bounds themselves do)
+    const bool up = t & 2, odd = t & 1;
+    float l[2], h[2];
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+        l[k] = fminf(up ? lo[k + 2] : lo[k], __shfl_xor_sync(0xffffffffu, up ? lo[k] : lo[k + 2], 2));
+        h[k] = fmaxf(up ? hi[k + 2] : hi[k], __shfl_xor_sync(0xffffffffu, up ? hi[k] : hi[k + 2], 2));
+    }
+    low = fminf(odd ? l[1] : l[0], __shfl_xor_sync(0xffffffffu, odd ? l[0] : l[1], 1));
+    high = fmaxf(odd ? h[1] : h[0], __shfl_xor_sync(0xffffffffu, odd ? h[0] : h[1], 1));
+}
+
+// s (low half) and m of a group.  A group of nothing but NaN holds zeros; columns beyond the largest float16 get the outermost codes.
+__device__ __forceinline__ uint32_t group_params(float low, float high) {
+    if (low != low) low = high = 0.f;
     low = fminf(fmaxf(low, -C4_MOST), C4_MOST);
     high = fminf(fmaxf(high, -C4_MOST), C4_MOST);
-    sh = group_step(low, high);
-    mh = __float2half_rn(low);
-    const float s = __half2float(sh), m = __half2float(mh);
-    const float inv = s > 0.f ? __frcp_rn(s) : 0.f;
-    constexpr float round_at = 12582912.f;  // 1.5 2^23: the sum is a whole number, to the nearest, ties to even
-    float code[8], off = 0.f;
+    return (uint32_t)__half_as_ushort(group_step(low, high)) | (uint32_t)__half_as_ushort(__float2half_rn(low)) << 16;
+}
+
+// The codes of eight columns, column n in bits 4 n.
+__device__ __forceinline__ uint32_t quantise8(const float (&x)[8], uint32_t params) {
+    const float2 sm = __half22float2(*reinterpret_cast<const __half2*>(&params));
+    const float s = sm.x, m = sm.y, inv = s > 0.f ? fast_rcp(s) : 0.f, inv15 = inv * (1.f / 15.f);
+    // the quotient over 15, kept within 0 .. 1 (NaN: 0); 1.5 2^23 + 15 times that is a whole number, to the nearest, ties to even
+    constexpr float round_at = 12582912.f;
+    const float2 minus_m = make_float2(-m, -m), fifteen = make_float2(15.f, 15.f), to_whole = make_float2(round_at, round_at),
+                 back = make_float2(-round_at, -round_at), minus = make_float2(-1.f, -1.f);
+    float2 code[4];
+    float off = 0.f;
 #pragma unroll
-    for (int n = 0; n < 8; ++n) {
-        const float q = fminf(fmaxf((x[n] - m) * inv, 0.f), 15.f);  // (NaN: 0)
-        code[n] = __fadd_rn(__fadd_rn(q, round_at), -round_at);
-        off = fmaxf(off, fabsf(q - code[n]));
+    for (int n = 0; n < 4; ++n) {
+        const float2 d = __fadd2_rn(make_float2(x[2 * n], x[2 * n + 1]), minus_m);
+        const float2 q = make_float2(__saturatef(d.x * inv15), __saturatef(d.y * inv15));
+        code[n] = __fadd2_rn(__ffma2_rn(q, fifteen, to_whole), back);
+        const float2 e = __ffma2_rn(code[n], minus, __fmul2_rn(q, fifteen));
+        off = fmaxf(off, fmaxf(fabsf(e.x), fabsf(e.y)));
     }
-    // The quotient in float32 is off by less than 1e-5: next to a border between two codes it is taken in 64 bits.
+    // The quotient in float32 is off by less than 1e-5: what lies that near to a border k + 1/2 between two codes is compared with it in
+    // 64 bits, where x - m and (k + 1/2) s have room.  (Types of few bits come here often: (x - m) / s is a ratio of small numbers, and of
+    // 256 bf16 columns one lies on a border in a seventh of the cases.)
     if (off > 0.5f - 2e-5f) {
 #pragma unroll
         for (int n = 0; n < 8; ++n) {
-            const double q = ((double)x[n] - (double)m) / (double)s;
-            code[n] = (float)fmin(fmax(rint(q), 0.0), 15.0);
+            float& c = n & 1 ? code[n >> 1].y : code[n >> 1].x;
+            const float q = fminf(fmaxf((x[n] - m) * inv, 0.f), 15.f);
+            if (fabsf(q - c) > 0.5f - 4e-5f) {
+                const float below = floorf(q);
+                const double d = fma(-((double)below + 0.5), (double)s, (double)x[n] - (double)m);
+                c = below + (d > 0.0 || (d == 0.0 && ((int)below & 1)) ? 1.f : 0.f);
+            }
         }
     }
     // (four codes are a number below 2^16, which the sum with 2^23 has in its low bits)
     uint32_t half[2];
 #pragma unroll
     for (int k = 0; k < 2; ++k) {
-        const float* c = code + 4 * k;
-        half[k] = __float_as_uint(fmaf(fmaf(fmaf(c[3], 16.f, c[2]), 16.f, c[1]), 16.f, c[0]) + 8388608.f);
+        const float2 c0 = code[2 * k], c1 = code[2 * k + 1];
+        half[k] = __float_as_uint(fmaf(fmaf(fmaf(c1.y, 16.f, c1.x), 16.f, c0.y), 16.f, c0.x) + 8388608.f);
     }
     return __byte_perm(half[0], half[1], 0x5410);
 }
 
 template <typename T>
-__global__ void __launch_bounds__(C4_THREADS) cache4_store_kernel(const __grid_constant__ Cache4Store p) {
+__global__ void __launch_bounds__(C4_THREADS, 4) cache4_store_kernel(const __grid_constant__ Cache4Store p) {
     pdl_wait();
     pdl_trigger();
     const uint32_t u = blockIdx.x * C4_THREADS + threadIdx.x;
@@ -122,10 +155,18 @@ __global__ void __launch_bounds__(C4_THREADS) cache4_store_kernel(const __grid_c
             for (int n = 0; n < 8; ++n) x[k][n] = 0.f;
         }
     }
+    float low, high;
+    group_bounds(x, c8 & 3, low, high);
+    const uint32_t own = group_params(low, high);
     uint32_t word[4];
     __half s[4], m[4];
 #pragma unroll
-    for (int k = 0; k < 4; ++k) word[k] = quantise8(x[k], s[k], m[k]);
+    for (int k = 0; k < 4; ++k) {
+        const uint32_t params = __shfl_sync(0xffffffffu, own, (threadIdx.x & 28) + k);
+        word[k] = quantise8(x[k], params);
+        s[k] = __ushort_as_half((unsigned short)params);
+        m[k] = __ushort_as_half((unsigned short)(params >> 16));
+    }
     if (!on || from >= to) return;
     const Place w(p.c, part, b, h, quad, c8);
     const bool whole = from == 0 && to == 4, first = (c8 & 3) == 0;

@@ -673,7 +673,7 @@ static Attend4Plan attend4_plan(const Cache4View& c, int dtype, int heads, int s
     static const char* dbg = getenv("A4S");
     if (dbg) splits = atoi(dbg) < most ? atoi(dbg) : most;
     a.splits = (int)splits;
-    a.bytes = splits <= A4_CLUSTER ? 16 : (size_t)c.batch * c.kv_heads * rows * splits * (c.dim + 4) * sizeof(float);
+    a.bytes = splits <= A4_CLUSTER ? 0 : (size_t)c.batch * c.kv_heads * rows * splits * (c.dim + 4) * sizeof(float);
     return a;
 }
 
@@ -717,7 +717,7 @@ size_t rotor_b200_cache4_attend_workspace_bytes(const rotor_b200_cache4* cache, 
     if (attend4_check(cache, c, dtype, heads, seq, longest, window)) return 0;
     const size_t a = attend4_plan(c, dtype, heads, seq, longest, window, true).bytes;
     const size_t b = attend4_plan(c, dtype, heads, seq, longest, window, false).bytes;
-    return a > b ? a : b;
+    return a > b ? a : b > 16 ? b : 16;
 }
 
 int rotor_b200_cache4_attend(const rotor_b200_cache4* cache, const void* q, int dtype, const int64_t* q_strides_host, int heads, int seq,
@@ -725,14 +725,14 @@ int rotor_b200_cache4_attend(const rotor_b200_cache4* cache, const void* q, int 
                              void* workspace, size_t workspace_bytes, void* stream) {
     Attend4 a;
     if (const int e = attend4_check(cache, a.c, dtype, heads, seq, longest, window)) return e;
-    RB_REQUIRE(q && q_strides_host && out && workspace && past >= 0 && (past_len || past <= a.c.max_seq - seq));
+    RB_REQUIRE(q && q_strides_host && out && past >= 0 && (past_len || past <= a.c.max_seq - seq));
     const int64_t* s = q_strides_host;
     const int size = dtype == ROTOR_B200_F32 ? 4 : 2;
     RB_REQUIRE(s[0] >= 0 && s[1] >= 0 && s[2] >= 0 && (uintptr_t)q % size == 0 && (((uintptr_t)out | (uintptr_t)workspace) & 15) == 0);
     a.wide = (((uintptr_t)q | (uintptr_t)((s[0] | s[1] | s[2]) * size)) & 15) == 0;
     a.past = Past{past_len, past, longest < a.c.max_seq ? longest : a.c.max_seq};
     const Attend4Plan plan = attend4_plan(a.c, dtype, heads, seq, past_len ? longest : past, window, a.wide);
-    if (plan.bytes > workspace_bytes) return ROTOR_B200_ERR_WORKSPACE;
+    if (plan.bytes > workspace_bytes || (plan.bytes && !workspace)) return ROTOR_B200_ERR_WORKSPACE;
     const cudaStream_t st = as_stream(stream);
     if (plan.prompt) {
         Cache4Expand x;

@@ -18,7 +18,7 @@ DECODER_LIB_PATH = os.path.join(_HERE, "librotor_b200_decoder.so")
 
 OK = 0
 VARIANT_AUTO, VARIANT_DP4A, VARIANT_MMA = 0, 1, 2
-ERR_TOO_LARGE = 6
+ERR_WORKSPACE, ERR_TOO_LARGE = 4, 6
 STATIC_SCRATCH_BYTES = 4 << 20
 
 
@@ -185,7 +185,7 @@ _c4p, _i64, _sdp = C.POINTER(Cache4), C.c_int64, C.POINTER(C.c_int64)
 _SIGNATURES.update({
     "rotor_b200_beam_select_workspace_bytes": (_sz, [_i, _i, _i, _i]),
     "rotor_b200_beam_select": (_i, [_p, _i, _i64, _i64, _p, _p, _i, _i, _i, _i, _i64, _p, _p, _p, _p, _sz, _p]),
-    "rotor_b200_reorder_states": (_i, [C.POINTER(State), _i, _p, _i, _i, _p]),
+    "rotor_b200_reorder_states": (_i, [_p, _i, _p, _i, _i, _p]),
     "rotor_b200_cache4_append": (_i, [_c4p, _p, _p, _i, _sdp, _sdp, _i, _i, _p, _p]),
     "rotor_b200_cache4_read": (_i, [_c4p, _i, _i, _p, _p, _i, _p]),
     "rotor_b200_cache4_attend_workspace_bytes": (_sz, [_c4p, _i, _i, _i, _i, _i]),
@@ -230,6 +230,12 @@ def stream():
     """The current stream of the current device, as the address that the C ABI takes."""
     torch = require_cuda()
     return _current_stream(torch.cuda.current_device())
+
+
+def device_and_stream():
+    """The current device's number and its current stream's address."""
+    device = require_cuda().cuda.current_device()
+    return device, _current_stream(device)
 
 
 def _stream_lookup(torch):

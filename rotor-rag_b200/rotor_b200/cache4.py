@@ -9,10 +9,11 @@ from __future__ import annotations
 import ctypes as C
 
 from . import abi
-from .abi import RotorB200Error, check, lib
+from .abi import check, lib
 from .ops import on_device, reorder_states, type_code
 
 GROUP = 32
+_Strides = C.c_int64 * 3
 DIMS = (32, 64, 96, 128, 192, 256)
 
 
@@ -50,11 +51,10 @@ class Cache4:
         ``length`` positions (all of them unless given)."""
         reorder_states(self.states(), beams, None if length is None else min(-(-length // 16) * 16, self.max_seq))
 
-    def _past(self, past, seq):
+    def _past(self, past, seq, device):
         """(number, address of the lengths or None), checked."""
         if hasattr(past, "data_ptr"):
-            import torch
-            on_device("past", past, 1, torch.int32)
+            on_device("past", past, device, 1, abi._torch.int32)
             if past.shape[0] != self.batch or not past.is_contiguous():
                 raise ValueError(f"past of shape {tuple(past.shape)} for {self.batch} sequences")
             if seq > self.max_seq:
@@ -64,39 +64,44 @@ class Cache4:
             raise ValueError(f"positions {past} to {past + seq} in a cache of {self.max_seq}")
         return past, None
 
-    def _rows(self, name, x, heads):
+    def _rows(self, name, x, heads, device):
         """Strides of rows [batch, seq, heads, dim], checked."""
-        on_device(name, x, 4)
+        on_device(name, x, device, 4)
         b, s, h, d = x.shape
         if b != self.batch or h != heads or d != self.dim:
             raise ValueError(f"{name} of shape {(b, s, h, d)}, expected {(self.batch, 'positions', heads, self.dim)}")
         sb, ss, sh, sd = x.stride()
         if sd != 1:
             raise ValueError(f"the columns of {name} have to lie side by side")
-        return (C.c_int64 * 3)(sb, ss, sh)
+        return _Strides(sb, ss, sh)
 
     def append(self, k, v, past):
         """Rows k and v [batch, seq, kv_heads, dim] (float32, bfloat16 or float16, any strides with columns side by side) are quantised
         into the positions from ``past`` on; with a tensor of lengths, positions behind the end of the cache are left out."""
-        ks, vs = self._rows("k", k, self.kv_heads), self._rows("v", v, self.kv_heads)
-        if k.shape != v.shape or k.dtype is not v.dtype:
+        device, stream = abi.device_and_stream()
+        ks, vs = self._rows("k", k, self.kv_heads, device), self._rows("v", v, self.kv_heads, device)
+        seq = k.shape[1]
+        if seq != v.shape[1] or k.dtype is not v.dtype:
             raise ValueError(f"k is {k.dtype} {tuple(k.shape)}, v is {v.dtype} {tuple(v.shape)}")
-        code, seq = type_code(k.dtype), k.shape[1]
-        number, lengths = self._past(past, seq)
+        code = type_code(k.dtype)
+        number, lengths = self._past(past, seq, device)
         if seq:
-            check(lib.rotor_b200_cache4_append(self._ref, k.data_ptr(), v.data_ptr(), code, ks, vs, seq, number, lengths, abi.stream()),
-                  "cache4_append")
+            status = lib.rotor_b200_cache4_append(self._ref, k.data_ptr(), v.data_ptr(), code, ks, vs, seq, number, lengths, stream)
+            if status:
+                check(status, "cache4_append")
 
     def read(self, begin: int, end: int, dtype=None):
         """What positions begin .. end - 1 stand for: keys and values [batch, kv_heads, end - begin, dim] (float32 unless told)."""
-        torch = abi.require_cuda()
-        dtype = dtype or torch.float32
+        _, stream = abi.device_and_stream()
+        dtype = dtype or abi._torch.float32
         if not 0 <= begin <= end <= self.max_seq:
             raise ValueError(f"positions {begin} to {end} of a cache of {self.max_seq}")
         code, shape = type_code(dtype), (self.batch, self.kv_heads, end - begin, self.dim)
-        k, v = torch.empty(shape, dtype=dtype, device="cuda"), torch.empty(shape, dtype=dtype, device="cuda")
+        k, v = self.k_step.new_empty(shape, dtype=dtype), self.k_step.new_empty(shape, dtype=dtype)
         if end > begin:
-            check(lib.rotor_b200_cache4_read(self._ref, begin, end, k.data_ptr(), v.data_ptr(), code, abi.stream()), "cache4_read")
+            status = lib.rotor_b200_cache4_read(self._ref, begin, end, k.data_ptr(), v.data_ptr(), code, stream)
+            if status:
+                check(status, "cache4_read")
         return k, v
 
     def attend(self, q, past, *, scale=None, window: int = 0, sinks=None, longest=None):
@@ -107,29 +112,34 @@ class Cache4:
         query sees that many positions, its own included.  ``sinks`` float32 [heads]: exp(sink) joins the softmax's denominator.
         ``longest``: with a tensor of lengths, the most that a sequence holds, by which the work is divided (the cache's size unless
         given); longer lengths are taken as it.  A query that sees no position gives zeros."""
-        torch = abi.require_cuda()
+        device, stream = abi.device_and_stream()
         heads = q.shape[2] if q.dim() == 4 else 0
-        strides = self._rows("q", q, heads)
+        strides = self._rows("q", q, heads, device)
         if heads < 1 or heads % self.kv_heads:
             raise ValueError(f"{heads} query heads cannot share {self.kv_heads} key/value heads evenly")
         code, seq = type_code(q.dtype), q.shape[1]
-        number, lengths = self._past(past, seq)
+        number, lengths = self._past(past, seq, device)
         if window < 0:
             raise ValueError(f"a window of {window} positions")
         if sinks is not None:
-            on_device("sinks", sinks, 1, torch.float32)
+            on_device("sinks", sinks, device, 1, abi._torch.float32)
             if sinks.shape[0] != heads or not sinks.is_contiguous():
                 raise ValueError("one sink per query head is needed")
-        out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+            sinks = sinks.data_ptr()
+        out = q.new_empty(q.shape)
         if seq == 0:
             return out
         bound = number if lengths is None else self.max_seq if longest is None else min(max(int(longest), 0), self.max_seq)
-        need = lib.rotor_b200_cache4_attend_workspace_bytes(self._ref, code, heads, seq, bound, window)
-        if need == 0:
-            raise RotorB200Error(f"{seq} queries of {heads} heads are beyond the attention's sizes")
-        workspace = torch.empty(need, dtype=torch.uint8, device=q.device)
-        check(lib.rotor_b200_cache4_attend(self._ref, q.data_ptr(), code, strides, heads, seq, number, lengths, bound,
-                                           self.dim ** -0.5 if scale is None else float(scale), window,
-                                           None if sinks is None else sinks.data_ptr(), out.data_ptr(), workspace.data_ptr(), need,
-                                           abi.stream()), "cache4_attend")
+        scale = self.dim ** -0.5 if scale is None else float(scale)
+
+        def call(workspace, size):
+            return lib.rotor_b200_cache4_attend(self._ref, q.data_ptr(), code, strides, heads, seq, number, lengths, bound, scale, window, sinks,
+                                                out.data_ptr(), workspace, size, stream)
+        status = call(None, 0)
+        if status == abi.ERR_WORKSPACE:      # (nothing has been launched; few tokens need none)
+            need = lib.rotor_b200_cache4_attend_workspace_bytes(self._ref, code, heads, seq, bound, window)
+            workspace = q.new_empty(need, dtype=abi._torch.uint8)
+            status = call(workspace.data_ptr(), need)
+        if status:
+            check(status, "cache4_attend")
         return out

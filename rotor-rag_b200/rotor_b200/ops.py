@@ -3,6 +3,8 @@ function here allocates its outputs with torch and hands raw pointers to
 librotor_b200.so on the current CUDA stream."""
 from __future__ import annotations
 
+import struct
+
 import numpy as np
 
 from . import abi
@@ -169,6 +171,7 @@ def sample(logits, mode, top_k=50, top_p=0.9, temperature=1.0, seed=0, counter=0
 
 
 # ------------------------------------------------------------------ beam search
+# (calls of one token or one request are bound by the host: what Python does in them is kept short)
 _CODES = {}
 
 
@@ -183,15 +186,14 @@ def type_code(dtype):
     return code
 
 
-def on_device(name, t, dim=None, dtype=None):
-    """The tensor, checked: on the current CUDA device, of that many dimensions and that type."""
-    if not t.is_cuda or t.get_device() != _torch().cuda.current_device():
+def on_device(name, t, device, dim=None, dtype=None):
+    """The tensor is on that CUDA device, of that many dimensions and that type."""
+    if t.get_device() != device:
         raise ValueError(f"{name} is on {t.device}, not on the current CUDA device")
     if dim is not None and t.dim() != dim:
         raise ValueError(f"{name} of shape {tuple(t.shape)} where {dim} dimensions are expected")
     if dtype is not None and t.dtype is not dtype:
         raise ValueError(f"{name} is {t.dtype}, expected {dtype}")
-    return t
 
 
 def beam_select(logits, scores, count, ended=None, pad=0):
@@ -203,59 +205,45 @@ def beam_select(logits, scores, count, ended=None, pad=0):
     ones the lower beam, then the lower token comes first.  ``ended`` bool [groups, width]: such a beam offers itself alone, as
     token ``pad`` with its score unchanged.  Logits of -inf or NaN, rows that hold +inf and beams whose score is not finite offer
     nothing; places that no candidate is left for hold -inf and the lowest unused (beam, token).  Up to 32 beams and 64 continuations."""
-    torch = _torch()
-    on_device("logits", logits, 3)
+    device, stream = abi.device_and_stream()
+    torch = abi._torch
+    on_device("logits", logits, device, 3)
+    on_device("scores", scores, device, 2, torch.float32)
     groups, width, vocab = logits.shape
-    code = type_code(logits.dtype)
-    on_device("scores", scores, 2, torch.float32)
-    if scores.shape != (groups, width):
+    group_stride, beam_stride, side_by_side = logits.stride()
+    code, count = type_code(logits.dtype), int(count)
+    if tuple(scores.shape) != (groups, width):
         raise ValueError(f"scores of shape {tuple(scores.shape)}, expected {(groups, width)}")
-    if vocab > 1 and logits.stride(2) != 1:
+    if side_by_side != 1 and vocab > 1:
         raise ValueError("the logits of a row have to lie side by side")
-    count = int(count)
     if not (1 <= width <= 32 and 1 <= count <= 64 and count <= width * vocab < 2 ** 31 and vocab <= 2 ** 30):
         raise ValueError(f"{count} of {width} x {vocab} candidates: up to 32 beams and 64 continuations, not more than there are")
     if ended is not None:
-        on_device("ended", ended, 2, torch.bool)
-        if ended.shape != (groups, width):
+        on_device("ended", ended, device, 2, torch.bool)
+        if tuple(ended.shape) != (groups, width):
             raise ValueError(f"ended of shape {tuple(ended.shape)}, expected {(groups, width)}")
         if not 0 <= pad < vocab:
             raise ValueError(f"padding token {pad} of {vocab}")
         ended = ended.contiguous()
     scores = scores.contiguous()
-    best = scores.new_empty((groups, count))
-    beams, tokens = torch.empty((2, groups, count), dtype=torch.int64, device=logits.device)
+    shape = (groups, count)
+    best = scores.new_empty(shape)
+    beams, tokens = scores.new_empty(shape, dtype=torch.int64), scores.new_empty(shape, dtype=torch.int64)
     if groups == 0:
         return best, beams, tokens
     need = lib.rotor_b200_beam_select_workspace_bytes(groups, width, vocab, count)
     if need == 0:
         raise RotorB200Error(f"{groups} groups of {width} beams: up to 65535 beams in a call")
-    workspace = torch.empty(need, dtype=torch.uint8, device=logits.device)
-    check(lib.rotor_b200_beam_select(logits.data_ptr(), code, logits.stride(0), logits.stride(1), scores.data_ptr(), ptr(ended), groups, width,
-                                     vocab, count, int(pad), best.data_ptr(), beams.data_ptr(), tokens.data_ptr(), workspace.data_ptr(), need,
-                                     abi.stream()), "beam_select")
+    workspace = scores.new_empty(need, dtype=torch.uint8)
+    status = lib.rotor_b200_beam_select(logits.data_ptr(), code, group_stride, beam_stride, scores.data_ptr(),
+                                        None if ended is None else ended.data_ptr(), groups, width, vocab, count, int(pad), best.data_ptr(),
+                                        beams.data_ptr(), tokens.data_ptr(), workspace.data_ptr(), need, stream)
+    if status:
+        check(status, "beam_select")
     return best, beams, tokens
 
 
-def _state(t, axis, length):
-    """The C ABI's description of what moves of a state."""
-    on_device("state", t)
-    size = t.element_size()
-    if t.dim() < 1 or not t[0].is_contiguous() or (t.shape[0] > 1 and t.stride(0) < t[0].numel()):
-        raise ValueError(f"a state's rows have to be contiguous and apart; got shape {tuple(t.shape)}, strides {t.stride()}")
-    row = t[0].numel() * size
-    s = abi.State(data=t.data_ptr(), row_stride=t.stride(0) * size, segment_stride=row, segment_bytes=row, segments=1)
-    if axis is not None and length is not None:
-        if not 1 <= axis < t.dim():
-            raise ValueError(f"positions along axis {axis} of a state of {t.dim()} dimensions")
-        if not 0 <= length <= t.shape[axis]:
-            raise ValueError(f"{length} positions of a state that holds {t.shape[axis]}")
-        inner = size
-        for n in t.shape[axis + 1:]:
-            inner *= n
-        s.segment_stride, s.segment_bytes = t.shape[axis] * inner, length * inner
-        s.segments = row // s.segment_stride
-    return s
+_STATE = struct.Struct("PNNNi4x")      # rotor_b200_state
 
 
 def reorder_states(states, beams, length=None):
@@ -264,23 +252,48 @@ def reorder_states(states, beams, length=None):
 
     ``states``: tensors [groups * width, ...] whose rows are contiguous, or pairs (tensor, axis) of which the first ``length`` positions
     along that axis move.  ``beams`` int64 [groups, width], up to 32 wide; rows whose beam is their own, or none of the group, stay."""
-    torch = _torch()
-    on_device("beams", beams, 2, torch.int64)
+    device, stream = abi.device_and_stream()
+    on_device("beams", beams, device, 2, abi._torch.int64)
     groups, width = beams.shape
+    rows = groups * width
     if width > 32:
         raise ValueError(f"{width} beams: up to 32")
-    described = []
+    described, addresses = [], set()
     for s in states:
         t, axis = s if isinstance(s, tuple) else (s, None)
-        if t.dim() < 1 or t.shape[0] != groups * width:
-            raise ValueError(f"a state of shape {tuple(t.shape)} for {groups} x {width} beams")
-        if t.numel():
-            described.append(_state(t, axis, length))
-    if len({s.data for s in described}) != len(described):
-        raise ValueError("the same state twice")
-    described = [s for s in described if s.segment_bytes]
+        shape, size = t.shape, t.element_size()
+        if t.get_device() != device:
+            raise ValueError(f"a state is on {t.device}, not on the current CUDA device")
+        if not shape or shape[0] != rows:
+            raise ValueError(f"a state of shape {tuple(shape)} for {groups} x {width} beams")
+        if axis is not None and length is not None:
+            if not 1 <= axis < len(shape):
+                raise ValueError(f"positions along axis {axis} of a state of {len(shape)} dimensions")
+            if not 0 <= length <= shape[axis]:
+                raise ValueError(f"{length} positions of a state that holds {shape[axis]}")
+        n = t.numel()
+        if n == 0:
+            continue
+        row = piece = part = n // rows * size
+        row_stride = row
+        if not t.is_contiguous():
+            row_stride = t.stride(0) * size
+            if not t[0].is_contiguous() or (rows > 1 and row_stride < row):
+                raise ValueError(f"a state's rows have to be contiguous and apart; got shape {tuple(shape)}, strides {t.stride()}")
+        if axis is not None and length is not None:
+            inner = size
+            for k in shape[axis + 1:]:
+                inner *= k
+            piece, part = shape[axis] * inner, length * inner
+        address = t.data_ptr()
+        if address in addresses:
+            raise ValueError("the same state twice")
+        addresses.add(address)
+        if part:
+            described.append(_STATE.pack(address, row_stride, piece, part, row // piece))
     if not described:
         return
     beams = beams.contiguous()
-    check(lib.rotor_b200_reorder_states((abi.State * len(described))(*described), len(described), beams.data_ptr(), groups, width,
-                                        abi.stream()), "reorder_states")
+    status = lib.rotor_b200_reorder_states(b"".join(described), len(described), beams.data_ptr(), groups, width, stream)
+    if status:
+        check(status, "reorder_states")

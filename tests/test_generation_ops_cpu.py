@@ -46,10 +46,12 @@ def test_calls_on_a_cache():
     def attend(q=A, dtype=0, s=strides(), heads=4, seq=1, past=0, longest=0, window=0, out=A, ws=A, size=1 << 30):
         return lib.rotor_b200_cache4_attend(c, q, dtype, s, heads, seq, past, None, longest, 1.0, window, None, out, ws, size, None)
     for kw in ({"q": None}, {"dtype": 7}, {"s": None}, {"s": strides(1, -1, 1)}, {"heads": 3}, {"heads": 0}, {"seq": 0}, {"seq": 33}, {"past": 32},
-               {"past": -1}, {"longest": -1}, {"window": -1}, {"out": None}, {"out": A + 4}, {"ws": None}, {"ws": A + 8}, {"q": A + 1}):
+               {"past": -1}, {"longest": -1}, {"window": -1}, {"out": None}, {"out": A + 4}, {"ws": A + 8}, {"q": A + 1}):
         assert attend(**kw) == ARG, kw
-    need = lib.rotor_b200_cache4_attend_workspace_bytes(c, 0, 4, 1, 5, 0)
-    assert need > 0 and attend(past=5, size=need - 1) == WORKSPACE
+    assert lib.rotor_b200_cache4_attend_workspace_bytes(c, 0, 4, 1, 5, 0) > 0
+    c = cache(max_seq=8192)
+    need = lib.rotor_b200_cache4_attend_workspace_bytes(c, 0, 4, 1, 8000, 0)
+    assert need > 0 and attend(past=8000, size=need - 1) == WORKSPACE and attend(past=8000, ws=None, size=0) == WORKSPACE
     assert attend(heads=65536) == SHAPE and lib.rotor_b200_cache4_attend_workspace_bytes(c, 0, 65536, 1, 5, 0) == 0
 
 
