@@ -20,16 +20,16 @@
 // Tiles travel by cp.async into a ring of the warp's own (no barrier, and the loads in flight do not depend on what the registers hold):
 // a tile of 128 columns is 2560 bytes, five copies a lane.
 #include <cmath>
-#include <cstdlib>
 
 #include "cache4.cuh"
 
 namespace rb {
 
-constexpr int A4_WARPS = 8, A4_THREADS = 32 * A4_WARPS;
 constexpr float A4_SLACK = 7.f;   // a new maximum below the old one plus this (in powers of two) leaves the shift where it is
 constexpr float A4_LIFT = 7.f;    // weights are at most 2^(lift + slack): p s below 2^15 for s below 2, and a smaller lift for larger s
 constexpr float A4_LOW = -1e30f;  // a shift that any score is above
+constexpr int A4_JOIN = 256;      // threads of the join
+constexpr int A4_SORTED = 128;    // most sequences that are taken by their length
 constexpr int A4_CLUSTER = 8;     // most splits that are joined inside a cluster
 
 struct Attend4 {
@@ -42,6 +42,7 @@ struct Attend4 {
     const float* sinks;
     Past past;
     int heads, group, seq, rows, window, splits;
+    int by_length;      // CTAs take the sequences from the longest to the shortest
     float scale2;       // scale log2(e)
 };
 
@@ -137,7 +138,7 @@ struct Tile4 {
     }
 };
 
-template <int NG, int R, int TERMS>
+template <int NG, int R, int TERMS, int W>
 struct A4Cfg {
     static constexpr int D = 32 * NG, Q = 8 * R;
     static constexpr int STAGES = NG >= 6 ? 2 : 3;
@@ -145,9 +146,9 @@ struct A4Cfg {
     static constexpr bool KEEP = NG * R * TERMS <= 4;  // the queries' operands stay in registers
     // queries as operands: per lane two pairs of a group's two steps of 16 columns; largest values and sums of the groups
     static constexpr int FRAG = 0, TOPS = FRAG + NG * TERMS * R * 512, SUMS = TOPS + NG * Q * 4, RING = SUMS + NG * Q * 4;
-    static constexpr int RING_BYTES = A4_WARPS * STAGES * Tile4<NG>::BYTES;
+    static constexpr int RING_BYTES = W * STAGES * Tile4<NG>::BYTES;
     // at the end, over the ring: sums of the warps' rows, shifts, masses; then the CTA's rows for the cluster
-    static constexpr int O = RING, SHIFT = O + A4_WARPS * Q * OS * 4, MASS = SHIFT + A4_WARPS * Q * 4, ROWS = MASS + A4_WARPS * Q * 4;
+    static constexpr int O = RING, SHIFT = O + W * Q * OS * 4, MASS = SHIFT + W * Q * 4, ROWS = MASS + W * Q * 4;
     static constexpr int END = ROWS + Q * OS * 4, SMEM = END > RING + RING_BYTES ? END : RING + RING_BYTES;
 };
 
@@ -196,19 +197,57 @@ __device__ __forceinline__ void finish4(const Attend4& p, int b, int hk, int row
     store4(p.out, p.dtype, (((size_t)b * p.seq + token) * p.heads + head) * p.c.dim + col, make_float4(y.x * inv, y.y * inv, y.z * inv, y.w * inv));
 }
 
-template <int NG, int R, int TERMS>
-__global__ void __launch_bounds__(A4_THREADS, NG* R <= 4 ? 2 : 1) attend4_kernel(const __grid_constant__ Attend4 p) {
-    using C = A4Cfg<NG, R, TERMS>;
+template <int NG, int R, int TERMS, int W>
+__global__ void __launch_bounds__(32 * W, (NG * R <= 4 ? 16 : 8) / W) attend4_kernel(const __grid_constant__ Attend4 p) {
+    using C = A4Cfg<NG, R, TERMS, W>;
+    constexpr int THREADS = 32 * W, OWN = (NG + W - 1) / W;  // groups whose query operands a warp makes
     using T = Tile4<NG>;
     constexpr int D = C::D, Q = C::Q, S = C::STAGES;
     extern __shared__ __align__(128) unsigned char a4_raw[];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
     const int blocks = (p.rows + Q - 1) / Q, block = blockIdx.x / p.splits, split = blockIdx.x - block * p.splits;
-    const int hk = block / blocks, r0 = (block - hk * blocks) * Q, b = blockIdx.y;
+    const int hk = block / blocks, r0 = (block - hk * blocks) * Q, last_row = min(r0 + Q, p.rows) - 1;
     pdl_wait();
     pdl_trigger();
+    int b = blockIdx.y;
+    if (p.by_length) {  // the longest sequences first: this CTA's is the one with blockIdx.y longer ones
+        int* lengths = reinterpret_cast<int*>(a4_raw + C::RING);
+        int& chosen = lengths[A4_SORTED];
+        int own = 0;
+        if (threadIdx.x < p.c.batch) lengths[threadIdx.x] = own = past_of(p.past, threadIdx.x);
+        __syncthreads();
+        if (threadIdx.x < p.c.batch) {
+            int longer = 0;
+            for (int i = 0; i < p.c.batch; ++i) longer += lengths[i] > own || (lengths[i] == own && i < (int)threadIdx.x);
+            if (longer == b) chosen = threadIdx.x;
+        }
+        __syncthreads();
+        b = chosen;
+        __syncthreads();  // (tiles are copied here next)
+    }
 
-    const int past = past_of(p.past, b), last_row = min(r0 + Q, p.rows) - 1;
+    // ---- queries: warp j loads group j (and j + W), which does not wait for the sequence's length
+    float qv[R][OWN][8];
+#pragma unroll
+    for (int h = 0; h < R; ++h) {
+        const int row = min(r0 + g + 8 * h, last_row), token = row / p.group, head = hk * p.group + row - token * p.group;
+        const size_t at = (size_t)b * p.qb + (size_t)token * p.qs + (size_t)head * p.qh + 8 * t;
+#pragma unroll
+        for (int k = 0; k < OWN; ++k) {
+            const int j = warp + k * W;
+            if (j < NG) {
+                if (p.dtype == ROTOR_B200_F32)
+                    load8(static_cast<const float*>(p.q) + at + 32 * j, p.wide, qv[h][k]);
+                else if (p.dtype == ROTOR_B200_BF16)
+                    load8(static_cast<const __nv_bfloat16*>(p.q) + at + 32 * j, p.wide, qv[h][k]);
+                else
+                    load8(static_cast<const __half*>(p.q) + at + 32 * j, p.wide, qv[h][k]);
+            }
+        }
+    }
+
+    // ---- the first tiles
+    const int past = past_of(p.past, b);
     const int pos0 = past + r0 / p.group, pos1 = past + last_row / p.group;  // positions of the block's first and last row
     const int seen0 = first_visible(pos0, 0, p.window), seen1 = min(pos1, p.c.max_seq - 1);  // what some row sees
     const int tile0 = seen0 / 16, tiles = max(seen1 / 16 + 1 - tile0, 0);
@@ -219,15 +258,15 @@ __global__ void __launch_bounds__(A4_THREADS, NG* R <= 4 ? 2 : 1) attend4_kernel
     const uint32_t ring_at = (uint32_t)__cvta_generic_to_shared(ring);
 #pragma unroll
     for (int s = 0; s < S - 1; ++s) {
-        if (first + s * A4_WARPS < end) source.fetch(first + s * A4_WARPS, ring_at + s * T::BYTES, lane);
+        if (first + s * W < end) source.fetch(first + s * W, ring_at + s * T::BYTES, lane);
         copy_commit();
     }
 
-    // ---- queries: warp j makes the operands of group j
+    // ---- the queries' operands
     uint4* frags = reinterpret_cast<uint4*>(a4_raw + C::FRAG);  // [j][term][h][lane]
     float(*tops)[Q] = reinterpret_cast<float(*)[Q]>(a4_raw + C::TOPS);
     float(*sums)[Q] = reinterpret_cast<float(*)[Q]>(a4_raw + C::SUMS);
-    float qv[R][8], fa[R][2];
+    float fa[R][2];
     int lo[R][2], hi[R][2];  // visible positions of query rows 2 t and 2 t + 1 (+ 8 h)
 #pragma unroll
     for (int h = 0; h < R; ++h) {
@@ -237,29 +276,25 @@ __global__ void __launch_bounds__(A4_THREADS, NG* R <= 4 ? 2 : 1) attend4_kernel
             lo[h][e] = first_visible(pos, 0, p.window);
             hi[h][e] = min(pos, p.c.max_seq - 1);  // (rows past the last one repeat it, and are not kept)
         }
-        if (warp < NG) {
-            const int row = min(r0 + g + 8 * h, last_row), token = row / p.group, head = hk * p.group + row - token * p.group;
-            const size_t at = (size_t)b * p.qb + (size_t)token * p.qs + (size_t)head * p.qh + 32 * warp + 8 * t;
-            if (p.dtype == ROTOR_B200_F32)
-                load8(static_cast<const float*>(p.q) + at, p.wide, qv[h]);
-            else if (p.dtype == ROTOR_B200_BF16)
-                load8(static_cast<const __nv_bfloat16*>(p.q) + at, p.wide, qv[h]);
-            else
-                load8(static_cast<const __half*>(p.q) + at, p.wide, qv[h]);
-            float top = 0.f, sum = 0.f;
 #pragma unroll
-            for (int n = 0; n < 8; ++n) {
-                top = fmaxf(top, fabsf(qv[h][n]));
-                sum += qv[h][n];
-            }
+        for (int k = 0; k < OWN; ++k) {
+            const int j = warp + k * W;
+            if (j < NG) {
+                float top = 0.f, sum = 0.f;
 #pragma unroll
-            for (int o = 1; o < 4; o <<= 1) {
-                top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-                sum += __shfl_xor_sync(0xffffffffu, sum, o);
-            }
-            if (t == 0) {
-                tops[warp][g + 8 * h] = top;
-                sums[warp][g + 8 * h] = sum;
+                for (int n = 0; n < 8; ++n) {
+                    top = fmaxf(top, fabsf(qv[h][k][n]));
+                    sum += qv[h][k][n];
+                }
+#pragma unroll
+                for (int o = 1; o < 4; o <<= 1) {
+                    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+                    sum += __shfl_xor_sync(0xffffffffu, sum, o);
+                }
+                if (t == 0) {
+                    tops[j][g + 8 * h] = top;
+                    sums[j][g + 8 * h] = sum;
+                }
             }
         }
     }
@@ -276,17 +311,21 @@ __global__ void __launch_bounds__(A4_THREADS, NG* R <= 4 ? 2 : 1) attend4_kernel
         const float fs = __int_as_float((127 + up) << 23), back = p.scale2 * __int_as_float((127 - up) << 23);
         fa[h][0] = __shfl_sync(0xffffffffu, back, 8 * t);
         fa[h][1] = __shfl_sync(0xffffffffu, back, 8 * t + 4);
-        if (warp < NG) {
-            float x[8];
 #pragma unroll
-            for (int n = 0; n < 8; ++n) x[n] = qv[h][n] * (n & 1 ? fs * 0.0625f : fs);
+        for (int k = 0; k < OWN; ++k) {
+            const int j = warp + k * W;
+            if (j < NG) {
+                float x[8];
 #pragma unroll
-            for (int term = 0; term < TERMS; ++term) {
-                const uint4 f = make_uint4(pack_half(x[0], x[4]), pack_half(x[2], x[6]), pack_half(x[1], x[5]), pack_half(x[3], x[7]));
-                frags[((warp * TERMS + term) * R + h) * 32 + lane] = f;
-                if (TERMS > 1) {
-                    const float2 a = half2_of(f.x), c = half2_of(f.y), d = half2_of(f.z), w = half2_of(f.w);
-                    x[0] -= a.x, x[4] -= a.y, x[2] -= c.x, x[6] -= c.y, x[1] -= d.x, x[5] -= d.y, x[3] -= w.x, x[7] -= w.y;
+                for (int n = 0; n < 8; ++n) x[n] = qv[h][k][n] * (n & 1 ? fs * 0.0625f : fs);
+#pragma unroll
+                for (int term = 0; term < TERMS; ++term) {
+                    const uint4 f = make_uint4(pack_half(x[0], x[4]), pack_half(x[2], x[6]), pack_half(x[1], x[5]), pack_half(x[3], x[7]));
+                    frags[((j * TERMS + term) * R + h) * 32 + lane] = f;
+                    if (TERMS > 1) {
+                        const float2 a = half2_of(f.x), c = half2_of(f.y), d = half2_of(f.z), w = half2_of(f.w);
+                        x[0] -= a.x, x[4] -= a.y, x[2] -= c.x, x[6] -= c.y, x[1] -= d.x, x[5] -= d.y, x[3] -= w.x, x[7] -= w.y;
+                    }
                 }
             }
         }
@@ -332,11 +371,11 @@ __global__ void __launch_bounds__(A4_THREADS, NG* R <= 4 ? 2 : 1) attend4_kernel
     // tiles that every row sees whole
     const int inner0 = (first_visible(pos1, 0, p.window) + 15) / 16, inner1 = (min(pos0, p.c.max_seq - 1) + 1) / 16;
     int stage = 0;
-    for (int tile = first; tile < end; tile += A4_WARPS) {
+    for (int tile = first; tile < end; tile += W) {
         copy_wait<S - 2>();
         __syncwarp();
         {
-            const int ahead = tile + (S - 1) * A4_WARPS;
+            const int ahead = tile + (S - 1) * W;
             const int into = stage == 0 ? S - 1 : stage - 1;
             if (ahead < end) source.fetch(ahead, ring_at + into * T::BYTES, lane);
             copy_commit();
@@ -545,15 +584,15 @@ __global__ void __launch_bounds__(A4_THREADS, NG* R <= 4 ? 2 : 1) attend4_kernel
     }
     __syncthreads();
     float* mine = reinterpret_cast<float*>(a4_raw + C::ROWS);  // [row][OS]: sums, shift, mass
-    for (int idx = threadIdx.x; idx < Q * (D / 4); idx += A4_THREADS) {
+    for (int idx = threadIdx.x; idx < Q * (D / 4); idx += THREADS) {
         const int r = idx / (D / 4), c4 = idx - r * (D / 4), row = r0 + r;
         if (row >= p.rows) break;
         float top = A4_LOW, total = 0.f;
 #pragma unroll
-        for (int w = 0; w < A4_WARPS; ++w) top = fmaxf(top, shifts[w][r]);
+        for (int w = 0; w < W; ++w) top = fmaxf(top, shifts[w][r]);
         float4 y = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
-        for (int w = 0; w < A4_WARPS; ++w) {
+        for (int w = 0; w < W; ++w) {
             const float f = fast_exp2(shifts[w][r] - top);
             const float4 v = *reinterpret_cast<const float4*>(all + (w * Q + r) * C::OS + 4 * c4);
             total = fmaf(f, masses[w][r], total);
@@ -575,7 +614,7 @@ __global__ void __launch_bounds__(A4_THREADS, NG* R <= 4 ? 2 : 1) attend4_kernel
     if (p.splits == 1 || p.splits > A4_CLUSTER) return;
     // the CTAs of a cluster are the splits of its rows: each finishes a share of them
     cluster_sync();
-    for (int idx = threadIdx.x * p.splits + split; idx < Q * (D / 4); idx += A4_THREADS * p.splits) {
+    for (int idx = threadIdx.x * p.splits + split; idx < Q * (D / 4); idx += THREADS * p.splits) {
         const int r = idx / (D / 4), c4 = idx - r * (D / 4), row = r0 + r;
         if (row >= p.rows) break;
         float2 sm[A4_CLUSTER];
@@ -604,13 +643,13 @@ __global__ void __launch_bounds__(A4_THREADS, NG* R <= 4 ? 2 : 1) attend4_kernel
 }
 
 // Joins the splits of a query row where they are more than a cluster: a CTA per row, its threads columns x shares of the splits.
-__global__ void __launch_bounds__(A4_THREADS) attend4_join_kernel(const __grid_constant__ Attend4 p) {
-    __shared__ float4 s_y[A4_THREADS];
-    __shared__ float s_mass[A4_THREADS];
+__global__ void __launch_bounds__(A4_JOIN) attend4_join_kernel(const __grid_constant__ Attend4 p) {
+    __shared__ float4 s_y[A4_JOIN];
+    __shared__ float s_mass[A4_JOIN];
     pdl_wait();
     pdl_trigger();
     const int D = p.c.dim, hk = blockIdx.x / p.rows, row = blockIdx.x - hk * p.rows, b = blockIdx.y;
-    const int shares = A4_THREADS / (D / 4), share = threadIdx.x / (D / 4), c = threadIdx.x - share * (D / 4);
+    const int shares = A4_JOIN / (D / 4), share = threadIdx.x / (D / 4), c = threadIdx.x - share * (D / 4);
     const float* part = p.part + ((size_t)(b * p.c.kv_heads + hk) * p.rows + row) * p.splits * (D + 4);
     float top = A4_LOW;
     for (int s = threadIdx.x & 31; s < p.splits; s += 32) top = fmaxf(top, __ldcg(part + (size_t)s * (D + 4) + D));
@@ -645,12 +684,12 @@ struct Attend4Plan {
     bool prompt;
     int span;                // prompt: dense rows of a head
     size_t dense_bytes;      // of the keys, and of the values
-    int splits, per_block;   // else: CTAs that share a row's positions, query rows of a block
+    int splits, per_block, by_length;  // else: CTAs that share a row's positions, query rows of a block, longest sequences first
     size_t bytes;            // of workspace
 };
 
 // For sequences that hold up to `longest` positions.
-static Attend4Plan attend4_plan(const Cache4View& c, int dtype, int heads, int seq, int longest, int window, bool wide) {
+static Attend4Plan attend4_plan(const Cache4View& c, int dtype, int heads, int seq, int longest, int window, bool wide, bool each_length) {
     Attend4Plan a = {};
     const int rows = seq * (heads / c.kv_heads), ng = c.dim / C4_GROUP;
     const int held = (int)((long long)longest + seq < c.max_seq ? longest + seq : c.max_seq);
@@ -665,37 +704,52 @@ static Attend4Plan attend4_plan(const Cache4View& c, int dtype, int heads, int s
     const int reach = window > 0 && held > (long long)window + seq ? window + seq : held;  // what the queries see between them
     a.per_block = rows > 8 && ng <= 4 ? 16 : 8;
     const long long blocks = (long long)c.batch * c.kv_heads * ((rows + a.per_block - 1) / a.per_block);
+    // Two CTAs (R NG > 4: one) are on an SM.  A CTA takes about 4 us beside its tiles (lengths and queries arrive, the warps' sums are joined), 0.7 more for a join inside a cluster and 3.5 for
+    // the join kernel; a tile of 128 columns of every warp about 0.9 us at the rate of the memory.
     const long long tiles = (reach + 15) / 16 + 1;
-    long long splits = (2LL * fused_sm_count() + blocks - 1) / blocks;
-    const long long most = (tiles + A4_WARPS - 1) / A4_WARPS;  // a tile per warp
-    if (splits > most) splits = most;
-    if (splits < 1) splits = 1;
-    static const char* dbg = getenv("A4S");
-    if (dbg) splits = atoi(dbg) < most ? atoi(dbg) : most;
-    a.splits = (int)splits;
+    const int slots = fused_sm_count() * (ng * a.per_block <= 32 ? 2 : 1);
+    const double tile_us = 0.9 * ng / 4;
+    double best = 1e30;
+    auto consider = [&](long long splits) {
+        if (splits < 1 || (splits - 1) * 8 >= tiles) return;
+        const double rounds = (double)((blocks * splits + slots - 1) / slots), each = (double)((tiles + splits * 8 - 1) / (splits * 8));
+        const double us = rounds * (4.0 + each * tile_us) + (splits == 1 ? 0.0 : splits <= A4_CLUSTER ? 0.7 : 3.5);
+        if (us < best) {
+            best = us;
+            a.splits = (int)splits;
+        }
+    };
+    a.splits = 1;
+    for (int splits = 1; splits <= A4_CLUSTER; ++splits) consider(splits);
+    for (int round = 1; round <= 2; ++round) consider(slots * round / blocks > A4_CLUSTER ? slots * round / blocks : 0);
+    consider(slots / blocks > A4_CLUSTER ? (tiles + 7) / 8 : 0);
+    a.by_length = each_length && c.batch <= A4_SORTED && blocks * a.splits > slots;
+    const long long splits = a.splits;
     a.bytes = splits <= A4_CLUSTER ? 0 : (size_t)c.batch * c.kv_heads * rows * splits * (c.dim + 4) * sizeof(float);
     return a;
 }
 
-template <int NG, int R, int TERMS>
-static int attend4_go(const Attend4& a, const Attend4Plan& plan, cudaStream_t st) {
-    constexpr int smem = A4Cfg<NG, R, TERMS>::SMEM;
+template <int NG, int R, int TERMS, int W>
+static int attend4_go(const Attend4& a, cudaStream_t st) {
+    constexpr int smem = A4Cfg<NG, R, TERMS, W>::SMEM;
     static PerDevice<bool> once;
     if (!once.here()) {
-        RB_CUDA(cudaFuncSetAttribute(attend4_kernel<NG, R, TERMS>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+        RB_CUDA(cudaFuncSetAttribute(attend4_kernel<NG, R, TERMS, W>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
         once.here() = true;
     }
-    const dim3 grid(a.c.kv_heads * ((a.rows + plan.per_block - 1) / plan.per_block) * a.splits, a.c.batch);
-    const int e = launch_chained(attend4_kernel<NG, R, TERMS>, grid, A4_THREADS, smem, st, a.splits <= A4_CLUSTER ? a.splits : 1, a);
-    return e || a.splits <= A4_CLUSTER ? e : launch_chained(attend4_join_kernel, dim3(a.rows * a.c.kv_heads, a.c.batch), A4_THREADS, 0, st, 1, a);
+    const bool cluster = a.splits > 1 && a.splits <= A4_CLUSTER;
+    const dim3 grid(a.c.kv_heads * ((a.rows + 8 * R - 1) / (8 * R)) * a.splits, a.c.batch);
+    const int e = launch_chained(attend4_kernel<NG, R, TERMS, W>, grid, 32 * W, smem, st, cluster ? a.splits : 1, a);
+    return e || a.splits <= A4_CLUSTER ? e : launch_chained(attend4_join_kernel, dim3(a.rows * a.c.kv_heads, a.c.batch), A4_JOIN, 0, st, 1, a);
 }
 
 template <int NG>
 static int attend4_pick(const Attend4& a, const Attend4Plan& plan, cudaStream_t st) {
     const bool f32 = a.dtype == ROTOR_B200_F32;
-    if constexpr (NG <= 4)
-        if (plan.per_block == 16) return f32 ? attend4_go<NG, 2, 2>(a, plan, st) : attend4_go<NG, 2, 1>(a, plan, st);
-    return f32 ? attend4_go<NG, 1, 2>(a, plan, st) : attend4_go<NG, 1, 1>(a, plan, st);
+    if constexpr (NG <= 4) {
+        if (plan.per_block == 16) return f32 ? attend4_go<NG, 2, 2, 8>(a, st) : attend4_go<NG, 2, 1, 8>(a, st);
+    }
+    return f32 ? attend4_go<NG, 1, 2, 8>(a, st) : attend4_go<NG, 1, 1, 8>(a, st);
 }
 
 static int attend4_check(const rotor_b200_cache4* cache, Cache4View& c, int dtype, int heads, int seq, int longest, int window) {
@@ -715,8 +769,8 @@ extern "C" {
 size_t rotor_b200_cache4_attend_workspace_bytes(const rotor_b200_cache4* cache, int dtype, int heads, int seq, int longest, int window) {
     Cache4View c;
     if (attend4_check(cache, c, dtype, heads, seq, longest, window)) return 0;
-    const size_t a = attend4_plan(c, dtype, heads, seq, longest, window, true).bytes;
-    const size_t b = attend4_plan(c, dtype, heads, seq, longest, window, false).bytes;
+    const size_t a = attend4_plan(c, dtype, heads, seq, longest, window, true, true).bytes;
+    const size_t b = attend4_plan(c, dtype, heads, seq, longest, window, false, true).bytes;
     return a > b ? a : b > 16 ? b : 16;
 }
 
@@ -731,7 +785,7 @@ int rotor_b200_cache4_attend(const rotor_b200_cache4* cache, const void* q, int 
     RB_REQUIRE(s[0] >= 0 && s[1] >= 0 && s[2] >= 0 && (uintptr_t)q % size == 0 && (((uintptr_t)out | (uintptr_t)workspace) & 15) == 0);
     a.wide = (((uintptr_t)q | (uintptr_t)((s[0] | s[1] | s[2]) * size)) & 15) == 0;
     a.past = Past{past_len, past, longest < a.c.max_seq ? longest : a.c.max_seq};
-    const Attend4Plan plan = attend4_plan(a.c, dtype, heads, seq, past_len ? longest : past, window, a.wide);
+    const Attend4Plan plan = attend4_plan(a.c, dtype, heads, seq, past_len ? longest : past, window, a.wide, past_len != nullptr);
     if (plan.bytes > workspace_bytes || (plan.bytes && !workspace)) return ROTOR_B200_ERR_WORKSPACE;
     const cudaStream_t st = as_stream(stream);
     if (plan.prompt) {
@@ -782,6 +836,7 @@ int rotor_b200_cache4_attend(const rotor_b200_cache4* cache, const void* q, int 
     a.rows = seq * a.group;
     a.window = window;
     a.splits = plan.splits;
+    a.by_length = plan.by_length;
     a.scale2 = scale * 1.4426950408889634f;
     switch (a.c.dim / C4_GROUP) {
         case 1: return attend4_pick<1>(a, plan, st);
