@@ -676,39 +676,32 @@ __global__ void __launch_bounds__(A4_JOIN) attend4_join_kernel(const __grid_cons
     finish4(p, b, hk, row, 4 * c, y, total, top);
 }
 
-// Query rows of a KV head from which 16-bit calls go to the prompt kernel: the cache's rows are made dense (bf16 or float16) in the workspace
-// first.
-constexpr int A4_PROMPT_ROWS = 192;
-
 struct Attend4Plan {
-    bool prompt;
+    bool prompt;             // the cache's rows are made dense (bf16 or float16) in the workspace, for the prompt kernel
     int span;                // prompt: dense rows of a head
     size_t dense_bytes;      // of the keys, and of the values
     int splits, per_block, by_length;  // else: CTAs that share a row's positions, query rows of a block, longest sequences first
     size_t bytes;            // of workspace
 };
 
-// For sequences that hold up to `longest` positions.
-static Attend4Plan attend4_plan(const Cache4View& c, int dtype, int heads, int seq, int longest, int window, bool wide, bool each_length) {
+// For sequences that hold up to `longest` positions (each its own number of them: `ragged`).  What is fastest goes by estimates in us:
+//   here      two CTAs (R NG > 4: one) are on an SM; a CTA takes about 4 us beside its tiles (lengths and queries arrive, the warps' sums are
+//             joined), 0.7 more for a join inside a cluster and 3.5 for the join kernel; a tile of 128 columns of every warp 0.9 us
+//             (the rate of the memory), of sixteen query rows, with a CTA on an SM, 0.75
+//   prompts   dense rows at about 5 TB/s and 3 us, then a CTA per 128 query rows, 7 us and 1.5 for every 128 keys
+// Measured here / as prompts, 16-bit types, heads of 128: 16 tokens of 4 sequences behind 2000 positions, 20/5 heads, 16.5 / 37 us;
+// 64 tokens 47 / 40; 16 tokens behind 16000 positions, 64/8 heads, 51 / 213; 64 tokens 231 / 215; 64 tokens of 32 sequences behind 1000
+// positions, 32/8 heads, 296 / 120.
+static Attend4Plan attend4_plan(const Cache4View& c, int dtype, int heads, int seq, int longest, int window, bool wide, bool ragged) {
     Attend4Plan a = {};
-    const int rows = seq * (heads / c.kv_heads), ng = c.dim / C4_GROUP;
+    const int group = heads / c.kv_heads, rows = seq * group, ng = c.dim / C4_GROUP, sms = fused_sm_count();
     const int held = (int)((long long)longest + seq < c.max_seq ? longest + seq : c.max_seq);
-    a.span = held;
-    a.prompt = wide && dtype != ROTOR_B200_F32 && rows >= A4_PROMPT_ROWS && prompt_attn_supported(c.batch, heads, c.kv_heads, c.dim, a.span) &&
-               (uint64_t)c.kv_heads * a.span * (c.dim / 8) <= 0x7fffff00u;
-    a.dense_bytes = round_up((size_t)c.batch * c.kv_heads * a.span * c.dim * 2, 256);
-    if (a.prompt) {
-        a.bytes = 2 * a.dense_bytes + (size_t)c.batch * sizeof(int);
-        return a;
-    }
     const int reach = window > 0 && held > (long long)window + seq ? window + seq : held;  // what the queries see between them
     a.per_block = rows > 8 && ng <= 4 ? 16 : 8;
-    const long long blocks = (long long)c.batch * c.kv_heads * ((rows + a.per_block - 1) / a.per_block);
-    // Two CTAs (R NG > 4: one) are on an SM.  A CTA takes about 4 us beside its tiles (lengths and queries arrive, the warps' sums are joined), 0.7 more for a join inside a cluster and 3.5 for
-    // the join kernel; a tile of 128 columns of every warp about 0.9 us at the rate of the memory.
-    const long long tiles = (reach + 15) / 16 + 1;
-    const int slots = fused_sm_count() * (ng * a.per_block <= 32 ? 2 : 1);
-    const double tile_us = 0.9 * ng / 4;
+    const long long blocks = (long long)c.batch * c.kv_heads * ((rows + a.per_block - 1) / a.per_block), tiles = (reach + 15) / 16 + 1;
+    const bool pair = ng * a.per_block <= 32;
+    const long long slots = sms * (pair ? 2 : 1);
+    const double tile_us = (pair ? 0.9 : 0.75) * ng / 4;
     double best = 1e30;
     auto consider = [&](long long splits) {
         if (splits < 1 || (splits - 1) * 8 >= tiles) return;
@@ -719,13 +712,26 @@ static Attend4Plan attend4_plan(const Cache4View& c, int dtype, int heads, int s
             a.splits = (int)splits;
         }
     };
-    a.splits = 1;
     for (int splits = 1; splits <= A4_CLUSTER; ++splits) consider(splits);
     for (int round = 1; round <= 2; ++round) consider(slots * round / blocks > A4_CLUSTER ? slots * round / blocks : 0);
     consider(slots / blocks > A4_CLUSTER ? (tiles + 7) / 8 : 0);
-    a.by_length = each_length && c.batch <= A4_SORTED && blocks * a.splits > slots;
-    const long long splits = a.splits;
-    a.bytes = splits <= A4_CLUSTER ? 0 : (size_t)c.batch * c.kv_heads * rows * splits * (c.dim + 4) * sizeof(float);
+
+    a.span = held;
+    a.dense_bytes = round_up((size_t)c.batch * c.kv_heads * a.span * c.dim * 2, 256);
+    if (wide && dtype != ROTOR_B200_F32 && rows > 16 && prompt_attn_supported(c.batch, heads, c.kv_heads, c.dim, a.span) &&
+        (uint64_t)c.kv_heads * a.span * (c.dim / 8) <= 0x7fffff00u) {
+        const double most = (reach + 127) / 128, mean = most - 0.5 * (seq < reach ? seq : reach) / 128;  // tiles of keys
+        const double dense = 3.0 + (double)c.batch * c.kv_heads * reach * c.dim * 5.25 * 1e-6 / 5.0;
+        const double ctas = (double)c.batch * c.kv_heads * ((seq + 128 / group - 1) / (128 / group));
+        const double one = 7.0 + 1.5 * most, all = ctas / sms * (7.0 + 1.5 * mean);
+        a.prompt = dense + (one > all ? one : all) < best;
+    }
+    if (a.prompt) {
+        a.bytes = 2 * a.dense_bytes + (size_t)c.batch * sizeof(int);
+        return a;
+    }
+    a.by_length = ragged && c.batch <= A4_SORTED && blocks * a.splits > slots;
+    a.bytes = a.splits <= A4_CLUSTER ? 0 : (size_t)c.batch * c.kv_heads * rows * a.splits * (c.dim + 4) * sizeof(float);
     return a;
 }
 

@@ -97,7 +97,8 @@ class Cache4:
         if not 0 <= begin <= end <= self.max_seq:
             raise ValueError(f"positions {begin} to {end} of a cache of {self.max_seq}")
         code, shape = type_code(dtype), (self.batch, self.kv_heads, end - begin, self.dim)
-        k, v = self.k_step.new_empty(shape, dtype=dtype), self.k_step.new_empty(shape, dtype=dtype)
+        k = self.k_step.new_empty(shape, dtype=dtype)
+        v = abi._torch.empty_like(k)
         if end > begin:
             status = lib.rotor_b200_cache4_read(self._ref, begin, end, k.data_ptr(), v.data_ptr(), code, stream)
             if status:
@@ -126,7 +127,7 @@ class Cache4:
             if sinks.shape[0] != heads or not sinks.is_contiguous():
                 raise ValueError("one sink per query head is needed")
             sinks = sinks.data_ptr()
-        out = q.new_empty(q.shape)
+        out = abi._torch.empty_like(q) if q.is_contiguous() else q.new_empty(q.shape)
         if seq == 0:
             return out
         bound = number if lengths is None else self.max_seq if longest is None else min(max(int(longest), 0), self.max_seq)

@@ -228,7 +228,8 @@ def beam_select(logits, scores, count, ended=None, pad=0):
     scores = scores.contiguous()
     shape = (groups, count)
     best = scores.new_empty(shape)
-    beams, tokens = scores.new_empty(shape, dtype=torch.int64), scores.new_empty(shape, dtype=torch.int64)
+    beams = scores.new_empty(shape, dtype=torch.int64)
+    tokens = torch.empty_like(beams)
     if groups == 0:
         return best, beams, tokens
     need = lib.rotor_b200_beam_select_workspace_bytes(groups, width, vocab, count)

@@ -6,7 +6,7 @@ and one more to the type asked for.  Attention is off by
  * the rounding of the weights: float16 (2^-11 at most, with the ratio to the sum of weights that are not rounded) of the weighted sums
    of |v| and of s code for 16-bit types, two terms (2^-21) for float32.  (s code, because a value is m + s code and the rounded weight
    p s multiplies the code alone: where m and s code cancel, p s code (1 + e) + p m = p v + e p s code.);
- * 16-bit calls of 192 and more query rows a KV head: keys, values and weights are rounded to the type, h = finfo(type).eps / 2 each, which
+ * 16-bit calls of more than 16 query rows a KV head: keys, values and weights may be rounded to the type, h = finfo(type).eps / 2 each, which
    is h of the weighted sum of |v| for the weights and for the values, and h of |q| |k| for a score, twice with the ratio to the sum;
  * scores: products accumulated in float32 over at most 256 columns and 8 groups, each addition off by 2^-23 of the sum of |q| |k|:
    fewer than 64 of them, so 2^-17 of it, which is the relative error of a weight, twice with the ratio to the sum."""
@@ -48,7 +48,7 @@ def check_attention(torch, got, want, size, reach, dtype, kv):
     half = torch.finfo(getattr(torch, dtype)).eps / 2
     weight = 2.0 ** -21 if dtype == "float32" else 2.0 ** -11
     score = 2.0 ** -16
-    if dtype != "float32" and want.shape[1] * want.shape[2] // kv >= 192 and want.shape[3] <= 128:
+    if dtype != "float32" and want.shape[1] * want.shape[2] // kv > 16 and want.shape[3] <= 128:
         weight, score = 2 * half, 2 * half + score
     bound = half * np.abs(want) + size * (weight + score * (reach[..., None] + 1)) + 1e-30
     err = np.abs(host(got) - want)
