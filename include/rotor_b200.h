@@ -423,14 +423,15 @@ int rotor_b200_sample(const float* logits, int rows, int vocab, int mode, int to
  *    `count` candidates are left, the rest is filled with -inf and the lowest (w, v) that are not among them.
  *    logits: `dtype` [groups][width][vocab], rows at group_stride and beam_stride elements; scores float32 [groups][width];
  *    width <= 32, count <= 64 and <= width * vocab, vocab <= 2^30, width * vocab < 2^31.  out_scores float32, out_beams and out_tokens int64,
- *    [groups][count].  workspace: rotor_b200_beam_select_workspace_bytes bytes, 16-byte aligned, contents of no matter.
+ *    [groups][count].  workspace: 16-byte aligned, contents of no matter, rotor_b200_beam_select_workspace_bytes bytes; calls that use
+ *    none (few logits) take NULL, and the others return ERR_WORKSPACE before anything is launched.
  *  reorder_states: row b * width + w of every state becomes what row b * width + beams[b][w] was, in place; rows whose beam is
  *    their own, or no index of the group, stay.  `states` is a HOST array; width <= 32. */
 #define ROTOR_B200_F32 0
 #define ROTOR_B200_BF16 1
 #define ROTOR_B200_F16 2
 
-size_t rotor_b200_beam_select_workspace_bytes(int groups, int width, int vocab, int count);
+size_t rotor_b200_beam_select_workspace_bytes(int dtype, int groups, int width, int vocab, int count);
 int rotor_b200_beam_select(const void* logits, int dtype, int64_t group_stride, int64_t beam_stride, const float* scores,
                            const uint8_t* ended, int groups, int width, int vocab, int count, int64_t pad, float* out_scores,
                            int64_t* out_beams, int64_t* out_tokens, void* workspace, size_t workspace_bytes, void* stream);

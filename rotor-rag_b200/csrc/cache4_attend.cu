@@ -152,29 +152,6 @@ struct A4Cfg {
     static constexpr int END = ROWS + Q * OS * 4, SMEM = END > RING + RING_BYTES ? END : RING + RING_BYTES;
 };
 
-__device__ __forceinline__ void cluster_sync() {
-    asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
-    asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
-}
-__device__ __forceinline__ uint32_t cluster_at(const float* local, unsigned rank) {
-    uint32_t a;
-    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"((uint32_t)__cvta_generic_to_shared(local)), "r"(rank));
-    return a;
-}
-__device__ __forceinline__ float2 cluster_load2(const float* local, unsigned rank) {
-    float2 v;
-    asm volatile("ld.shared::cluster.v2.f32 {%0, %1}, [%2];" : "=f"(v.x), "=f"(v.y) : "r"(cluster_at(local, rank)) : "memory");
-    return v;
-}
-__device__ __forceinline__ float4 cluster_load4(const float* local, unsigned rank) {
-    float4 v;
-    asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
-                 : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w)
-                 : "r"(cluster_at(local, rank))
-                 : "memory");
-    return v;
-}
-
 __device__ __forceinline__ void store4(void* out, int dtype, size_t at, float4 y) {
     if (dtype == ROTOR_B200_F32) {
         *reinterpret_cast<float4*>(static_cast<float*>(out) + at) = y;

@@ -183,7 +183,7 @@ class State(C.Structure):
 _c4p, _i64, _sdp = C.POINTER(Cache4), C.c_int64, C.POINTER(C.c_int64)
 
 _SIGNATURES.update({
-    "rotor_b200_beam_select_workspace_bytes": (_sz, [_i, _i, _i, _i]),
+    "rotor_b200_beam_select_workspace_bytes": (_sz, [_i, _i, _i, _i, _i]),
     "rotor_b200_beam_select": (_i, [_p, _i, _i64, _i64, _p, _p, _i, _i, _i, _i, _i64, _p, _p, _p, _p, _sz, _p]),
     "rotor_b200_reorder_states": (_i, [_p, _i, _p, _i, _i, _p]),
     "rotor_b200_cache4_append": (_i, [_c4p, _p, _p, _i, _sdp, _sdp, _i, _i, _p, _p]),

@@ -8,7 +8,7 @@ import struct
 import numpy as np
 
 from . import abi
-from .abi import RotorB200Error, lib, ptr, check
+from .abi import lib, ptr, check
 
 
 def _torch():
@@ -232,13 +232,17 @@ def beam_select(logits, scores, count, ended=None, pad=0):
     tokens = torch.empty_like(beams)
     if groups == 0:
         return best, beams, tokens
-    need = lib.rotor_b200_beam_select_workspace_bytes(groups, width, vocab, count)
-    if need == 0:
-        raise RotorB200Error(f"{groups} groups of {width} beams: up to 65535 beams in a call")
-    workspace = scores.new_empty(need, dtype=torch.uint8)
-    status = lib.rotor_b200_beam_select(logits.data_ptr(), code, group_stride, beam_stride, scores.data_ptr(),
-                                        None if ended is None else ended.data_ptr(), groups, width, vocab, count, int(pad), best.data_ptr(),
-                                        beams.data_ptr(), tokens.data_ptr(), workspace.data_ptr(), need, stream)
+    if groups * width > 65535:
+        raise ValueError(f"{groups} groups of {width} beams: up to 65535 beams in a call")
+    def call(workspace, size):
+        return lib.rotor_b200_beam_select(logits.data_ptr(), code, group_stride, beam_stride, scores.data_ptr(),
+                                          None if ended is None else ended.data_ptr(), groups, width, vocab, count, int(pad),
+                                          best.data_ptr(), beams.data_ptr(), tokens.data_ptr(), workspace, size, stream)
+    status = call(None, 0)
+    if status == abi.ERR_WORKSPACE:      # (nothing has been launched; few logits need none)
+        need = lib.rotor_b200_beam_select_workspace_bytes(code, groups, width, vocab, count)
+        workspace = scores.new_empty(need, dtype=torch.uint8)
+        status = call(workspace.data_ptr(), need)
     if status:
         check(status, "beam_select")
     return best, beams, tokens

@@ -56,16 +56,13 @@ def test_calls_on_a_cache():
 
 
 def test_selections():
-    def select(logits=A, dtype=0, gs=30, bs=10, scores=A, ended=None, groups=2, width=3, vocab=10, count=4, pad=0, out=A, ws=A, size=1 << 30):
-        return lib.rotor_b200_beam_select(logits, dtype, gs, bs, scores, ended, groups, width, vocab, count, pad, out, A, A, ws, size, None)
-    for kw in ({"logits": None}, {"dtype": 3}, {"gs": -1}, {"scores": None}, {"out": None}, {"ws": None}, {"ws": A + 8}, {"ended": A, "pad": 10},
+    def select(logits=A, dtype=0, gs=30, bs=10, scores=A, ended=None, groups=2, width=3, vocab=10, count=4, pad=0, out=A, ws=None):
+        return lib.rotor_b200_beam_select(logits, dtype, gs, bs, scores, ended, groups, width, vocab, count, pad, out, A, A, ws, 0, None)
+    for kw in ({"logits": None}, {"dtype": 3}, {"gs": -1}, {"scores": None}, {"out": None}, {"ws": A + 8}, {"ended": A, "pad": 10},
                {"ended": A, "pad": -1}, {"logits": A + 2}):
         assert select(**kw) == ARG, kw
     for kw in ({"groups": 0}, {"width": 33}, {"count": 0}, {"count": 65}, {"count": 31}, {"width": 3, "vocab": 2 ** 30}, {"groups": 30000}):
         assert select(**kw) == SHAPE, kw
-    need = lib.rotor_b200_beam_select_workspace_bytes(2, 3, 10, 4)
-    assert need > 0 and select(size=need - 1) == WORKSPACE
-    assert lib.rotor_b200_beam_select_workspace_bytes(2, 33, 10, 4) == 0
 
 
 def test_reorderings():
