@@ -10,7 +10,9 @@
 // higher by another 1/16), float32 queries are split into two terms (2^-22 of the value).  The weights p_j are rounded to float16 and so
 // are their products with s_jg (2^-12 each; the sum of weights takes them as rounded), in float32 calls both are two terms (2^-22).
 // Scores, maxima, sums and outputs are float32.  Matrix instructions cut their sums off instead of rounding them, which shows after many
-// of them in a row: float32 calls begin every tile's sums at zero and add them up outside.
+// of them in a row, and align their products as if a subnormal number had the smallest normal exponent: with codes in the lowest four bits
+// a sum is off by 1.7e-7 of its terms' size, four bits higher by 3e-9 (as with the codes as normal numbers).  float32 calls begin every
+// tile's sums at zero and add them up outside, and shift all codes to the higher place.
 //
 // A warp takes tiles of 16 positions and keeps eight (R = 1) or sixteen (R = 2) query rows of one KV head (row = token x query head of the
 // group).  Both products have the codes as their 16-row operand: S = K Q^T (positions x queries) and O^T = V^T P (columns x queries);
@@ -138,6 +140,15 @@ struct Tile4 {
     }
 };
 
+// Every fourth code of a word (of a pair of 16-bit words), as two float16 numbers: 2^-24 (codes 0 and 2) or 2^-20 (1 and 3) times the code;
+// EXACT: 2^-20 for all.
+template <bool EXACT, int I>
+__device__ __forceinline__ uint32_t codes_of(uint32_t w) {
+    if constexpr (EXACT) return (I == 0 ? w << 4 : I == 1 ? w : I == 2 ? w >> 4 : w >> 8) & 0x00f000f0u;
+    return (I < 2 ? w : w >> 8) & (I % 2 ? 0x00f000f0u : 0x000f000fu);
+}
+constexpr float A4_LOW_CODE = 16777216.f, A4_HIGH_CODE = 1048576.f;  // 2^24, 2^20
+
 template <int NG, int R, int TERMS, int W>
 struct A4Cfg {
     static constexpr int D = 32 * NG, Q = 8 * R;
@@ -177,6 +188,7 @@ __device__ __forceinline__ void finish4(const Attend4& p, int b, int hk, int row
 template <int NG, int R, int TERMS, int W>
 __global__ void __launch_bounds__(32 * W, (NG * R <= 4 ? 16 : 8) / W) attend4_kernel(const __grid_constant__ Attend4 p) {
     using C = A4Cfg<NG, R, TERMS, W>;
+    constexpr bool EXACT = TERMS > 1;
     constexpr int THREADS = 32 * W, OWN = (NG + W - 1) / W;  // groups whose query operands a warp makes
     using T = Tile4<NG>;
     constexpr int D = C::D, Q = C::Q, S = C::STAGES;
@@ -294,7 +306,7 @@ __global__ void __launch_bounds__(32 * W, (NG * R <= 4 ? 16 : 8) / W) attend4_ke
             if (j < NG) {
                 float x[8];
 #pragma unroll
-                for (int n = 0; n < 8; ++n) x[n] = qv[h][k][n] * (n & 1 ? fs * 0.0625f : fs);
+                for (int n = 0; n < 8; ++n) x[n] = qv[h][k][n] * (n & 1 && !EXACT ? fs * 0.0625f : fs);
 #pragma unroll
                 for (int term = 0; term < TERMS; ++term) {
                     const uint4 f = make_uint4(pack_half(x[0], x[4]), pack_half(x[2], x[6]), pack_half(x[1], x[5]), pack_half(x[3], x[7]));
@@ -389,15 +401,16 @@ __global__ void __launch_bounds__(32 * W, (NG * R <= 4 ? 16 : 8) / W) attend4_ke
 #pragma unroll
             for (int j = 0; j < NG; ++j) {
                 const uint32_t w0 = k0.w[j], w1 = k1.w[j];
-                const float f0 = s0.half_at(j) * 16777216.f, f1 = s1.half_at(j) * 16777216.f;
+                constexpr float unit = EXACT ? A4_HIGH_CODE : A4_LOW_CODE;
+                const float f0 = s0.half_at(j) * unit, f1 = s1.half_at(j) * unit;
 #pragma unroll
                 for (int h = 0; h < R; ++h) {
                     float acc[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
                     for (int term = TERMS - 1; term >= 0; --term) {
                         const uint4 f = frag(j, term, h);
-                        a4_mma(acc, w0 & 0x000f000fu, w1 & 0x000f000fu, w0 >> 8 & 0x000f000fu, w1 >> 8 & 0x000f000fu, f.x, f.y);
-                        a4_mma(acc, w0 & 0x00f000f0u, w1 & 0x00f000f0u, w0 >> 8 & 0x00f000f0u, w1 >> 8 & 0x00f000f0u, f.z, f.w);
+                        a4_mma(acc, codes_of<EXACT, 0>(w0), codes_of<EXACT, 0>(w1), codes_of<EXACT, 2>(w0), codes_of<EXACT, 2>(w1), f.x, f.y);
+                        a4_mma(acc, codes_of<EXACT, 1>(w0), codes_of<EXACT, 1>(w1), codes_of<EXACT, 3>(w0), codes_of<EXACT, 3>(w1), f.z, f.w);
                     }
                     sc[h][0] = fmaf(f0, acc[0], sc[h][0]);
                     sc[h][1] = fmaf(f0, acc[1], sc[h][1]);
@@ -514,18 +527,20 @@ __global__ void __launch_bounds__(32 * W, (NG * R <= 4 ? 16 : 8) / W) attend4_ke
                     const __half2 l0 = __hfma2(as_half2(pw[h][1][0]), s0, __hfma2(as_half2(pw[h][0][0]), s0, __hneg2(w0)));
                     const __half2 l1 = __hfma2(as_half2(pw[h][1][1]), s1, __hfma2(as_half2(pw[h][0][1]), s1, __hneg2(w1)));
                     float d[4] = {0.f, 0.f, 0.f, 0.f}, d2[4] = {0.f, 0.f, 0.f, 0.f};
-                    a4_mma(d, a & 0x000f000fu, a & 0x00f000f0u, c & 0x000f000fu, c & 0x00f000f0u, as_word(l0), as_word(l1));
-                    a4_mma(d2, a >> 8 & 0x000f000fu, a >> 8 & 0x00f000f0u, c >> 8 & 0x000f000fu, c >> 8 & 0x00f000f0u, as_word(l0), as_word(l1));
-                    a4_mma(d, a & 0x000f000fu, a & 0x00f000f0u, c & 0x000f000fu, c & 0x00f000f0u, as_word(w0), as_word(w1));
-                    a4_mma(d2, a >> 8 & 0x000f000fu, a >> 8 & 0x00f000f0u, c >> 8 & 0x000f000fu, c >> 8 & 0x00f000f0u, as_word(w0), as_word(w1));
+#pragma unroll
+                    for (int term = 1; term >= 0; --term) {
+                        const uint32_t b0 = as_word(term ? l0 : w0), b1 = as_word(term ? l1 : w1);
+                        a4_mma(d, codes_of<EXACT, 0>(a), codes_of<EXACT, 1>(a), codes_of<EXACT, 0>(c), codes_of<EXACT, 1>(c), b0, b1);
+                        a4_mma(d2, codes_of<EXACT, 2>(a), codes_of<EXACT, 3>(a), codes_of<EXACT, 2>(c), codes_of<EXACT, 3>(c), b0, b1);
+                    }
 #pragma unroll
                     for (int i = 0; i < 4; ++i) {
                         o[h][2 * j][i] += d[i];
                         o[h][2 * j + 1][i] += d2[i];
                     }
                 } else {
-                    a4_mma(o[h][2 * j], a & 0x000f000fu, a & 0x00f000f0u, c & 0x000f000fu, c & 0x00f000f0u, as_word(w0), as_word(w1));
-                    a4_mma(o[h][2 * j + 1], a >> 8 & 0x000f000fu, a >> 8 & 0x00f000f0u, c >> 8 & 0x000f000fu, c >> 8 & 0x00f000f0u, as_word(w0),
+                    a4_mma(o[h][2 * j], codes_of<EXACT, 0>(a), codes_of<EXACT, 1>(a), codes_of<EXACT, 0>(c), codes_of<EXACT, 1>(c), as_word(w0), as_word(w1));
+                    a4_mma(o[h][2 * j + 1], codes_of<EXACT, 2>(a), codes_of<EXACT, 3>(a), codes_of<EXACT, 2>(c), codes_of<EXACT, 3>(c), as_word(w0),
                            as_word(w1));
                 }
             }
@@ -550,9 +565,9 @@ __global__ void __launch_bounds__(32 * W, (NG * R <= 4 ? 16 : 8) / W) attend4_ke
         float* to = all + (warp * Q + r) * C::OS + 4 * g;
 #pragma unroll
         for (int j = 0; j < NG; ++j) {
-            // columns 32 j + 4 g .. + 3; sums of codes four bits higher are 16 times too large
+            // columns 32 j + 4 g .. + 3
             const float l0 = __shfl_sync(0xffffffffu, rest[h][0], 4 * j + t), l1 = __shfl_sync(0xffffffffu, rest[h][1], 4 * j + t);
-            constexpr float c0 = 16777216.f, c1 = 1048576.f;
+            constexpr float c0 = EXACT ? A4_HIGH_CODE : A4_LOW_CODE, c1 = A4_HIGH_CODE;
             const float(&a)[4] = o[h][2 * j], (&c)[4] = o[h][2 * j + 1];
             *reinterpret_cast<float4*>(to + 32 * j) = make_float4(fmaf(a[0], c0, l0), fmaf(a[2], c1, l0), fmaf(c[0], c0, l0), fmaf(c[2], c1, l0));
             *reinterpret_cast<float4*>(to + C::OS + 32 * j) =
