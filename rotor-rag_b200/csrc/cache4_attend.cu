@@ -689,7 +689,7 @@ static Attend4Plan attend4_plan(const Cache4View& c, int dtype, int heads, int s
     const int group = heads / c.kv_heads, rows = seq * group, ng = c.dim / C4_GROUP, sms = fused_sm_count();
     const int held = (int)((long long)longest + seq < c.max_seq ? longest + seq : c.max_seq);
     const int reach = window > 0 && held > (long long)window + seq ? window + seq : held;  // what the queries see between them
-    a.per_block = rows > 8 && ng <= 4 ? 16 : 8;
+    a.per_block = rows > 8 ? 16 : 8;
     const long long blocks = (long long)c.batch * c.kv_heads * ((rows + a.per_block - 1) / a.per_block), tiles = (reach + 15) / 16 + 1;
     const bool pair = ng * a.per_block <= 32;
     const long long slots = sms * (pair ? 2 : 1);
@@ -744,9 +744,7 @@ static int attend4_go(const Attend4& a, cudaStream_t st) {
 template <int NG>
 static int attend4_pick(const Attend4& a, const Attend4Plan& plan, cudaStream_t st) {
     const bool f32 = a.dtype == ROTOR_B200_F32;
-    if constexpr (NG <= 4) {
-        if (plan.per_block == 16) return f32 ? attend4_go<NG, 2, 2, 8>(a, st) : attend4_go<NG, 2, 1, 8>(a, st);
-    }
+    if (plan.per_block == 16) return f32 ? attend4_go<NG, 2, 2, 8>(a, st) : attend4_go<NG, 2, 1, 8>(a, st);
     return f32 ? attend4_go<NG, 1, 2, 8>(a, st) : attend4_go<NG, 1, 1, 8>(a, st);
 }
 

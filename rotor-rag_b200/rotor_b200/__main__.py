@@ -1,6 +1,6 @@
 """Command line: ``python -m rotor_b200 <command>``.
 
-  generate  --model DIR --prompt "1 2 3" [--prompt ...]   token ids in, token ids out
+  generate  --model DIR --prompt "1 2 3" [--prompt ...] [--beams N]   token ids in, token ids out
   trace     --model DIR --dtype D --out DIR [--max-tokens N]   replay steps from standard input
   info      [--model DIR]                                 known architectures; a model folder's choice
 """
@@ -16,7 +16,13 @@ def _generate(a):
     from .registry import load_model
     from .synth import PassThroughTokenizer
     longest = max(len(p.split()) for p in a.prompt) + a.max_new_tokens
-    model = load_model(a.model, dtype=a.dtype, max_seq=longest, max_batch=len(a.prompt))
+    if a.beams > 1 and (len(a.prompt) > 1 or a.sampling != "greedy"):
+        raise SystemExit("beams are searched behind one prompt, without sampling")
+    model = load_model(a.model, dtype=a.dtype, max_seq=longest, max_batch=max(len(a.prompt), a.beams))
+    if a.beams > 1:
+        for ids, score in model.generate_beams([int(t) for t in a.prompt[0].split()], a.beams, a.max_new_tokens):
+            print(f"{score:.6f}", " ".join(map(str, ids)))
+        return 0
     if len(a.prompt) > 1:
         if a.sampling != "greedy":
             raise SystemExit("several prompts are generated greedily as one batch")
@@ -62,6 +68,7 @@ def main(argv=None):
     g.add_argument("--prompt", action="append", required=True, help="token ids separated by spaces; repeat for a batch")
     g.add_argument("--max-new-tokens", type=int, default=32)
     g.add_argument("--sampling", default="greedy", choices=["greedy", "top-k", "top-p"])
+    g.add_argument("--beams", type=int, default=1, help="beam search: prints every beam's score and token ids, best first")
     g.add_argument("--top-k", type=int, default=50)
     g.add_argument("--top-p", type=float, default=0.9)
     g.add_argument("--temperature", type=float, default=1.0)

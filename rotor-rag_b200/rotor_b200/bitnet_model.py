@@ -162,6 +162,9 @@ class BitNetModel(HandleModel):
     def _caches(self, length, batch):
         return [KVCache(l.attention, length, batch) for l in self.layers]
 
+    def _cache_tensors(self):
+        return [t for l in self.layers for t in (l.attention.k_cache, l.attention.v_cache)]
+
     def _forward_hidden(self, h, ids_d, batch, seq, past):
         torch = abi.require_cuda()
         emb = self._embed[ids_d.reshape(-1)].float().contiguous()

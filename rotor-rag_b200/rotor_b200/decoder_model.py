@@ -422,3 +422,6 @@ class DecoderModel(HandleModel):
 
     def _caches(self, length, batch):
         return [KVCache(run, length, batch) for run in self.runs]
+
+    def _cache_tensors(self):
+        return [t for run in self.runs if run.source is None for t in (run.k_cache, run.v_cache) if t is not None]

@@ -25,6 +25,10 @@ class HandleModel:
     def _caches(self, length, batch):
         raise NotImplementedError
 
+    def _cache_tensors(self):
+        """The tensors that hold the cached positions, [sequence, head, position, column]."""
+        raise NotImplementedError
+
     def _forward_hidden(self, h, ids_d, batch, seq, past):
         raise NotImplementedError("this model family returns logits only")
 
@@ -211,6 +215,65 @@ class HandleModel:
                 out[:, 1:] = buf.T
         abi.device_status()
         return out
+
+    # -- beam search ---------------------------------------------------------------------------
+    def generate_beams(self, prompt_ids, width: int, max_new_tokens: int, eos: Optional[int] = None, length_penalty: float = 0.0):
+        """Beam search behind one prompt, or behind several of the same length: for each a list of ``width`` (token ids, score), best
+        first.
+
+        Every step the ``width`` best continuations of a prompt's beams go on (``ops.beam_select``), and the caches and the tokens so far
+        follow the beams they continue (``ops.reorder_states``).  A beam that takes ``eos`` has ended (the token is not part of the
+        result) and keeps its place as long as its score is among the best.  A score is the sum of the tokens' log-probabilities, that of
+        ``eos`` included; the results are ordered by score / tokens ** ``length_penalty``.  Up to 32 beams in all."""
+        torch = abi.require_cuda()
+        prompts = np.asarray(prompt_ids, dtype=np.int64)
+        single = prompts.ndim == 1
+        prompts = prompts.reshape(1, -1) if single else prompts
+        n, n_prompt = prompts.shape
+        rows = n * width
+        if n < 1 or n_prompt < 1 or not 1 <= width <= self.vocab_size or rows > 32:
+            raise ValueError(f"{n} prompts of {n_prompt} tokens with {width} beams each: up to 32 beams in all")
+        if eos is not None and not 0 <= eos < self.vocab_size:
+            raise ValueError(f"token {eos} of {self.vocab_size}")
+        if max_new_tokens <= 0:
+            found = [[([], 0.0)] * width for _ in range(n)]
+            return found[0] if single else found
+        self._ensure_handle(rows, 1, n_prompt + max_new_tokens)
+        h, stream = self._ensure_handle(n, n_prompt, n_prompt + max_new_tokens), abi.stream()
+
+        def logits_of(ids, batch, seq, past):
+            out = torch.empty((batch, self.vocab_size), dtype=torch.float32, device="cuda")
+            check(lib.rotor_b200_model_forward(h.h, ptr(ids), batch, seq, past, abi.LOGITS_LAST, ptr(out), None, stream), "model_forward")
+            return out
+
+        caches = [(t[:rows], 2) for t in self._cache_tensors()]
+        history = torch.zeros((rows, max_new_tokens), dtype=torch.int64, device="cuda")
+        logits = logits_of(ops.to_device(prompts), n, n_prompt, 0)
+        scores, beams, tokens = ops.beam_select(logits.view(n, 1, -1), torch.zeros((n, 1), device="cuda"), width)
+        # (prompt b ran in row b: its cache goes to the rows of its beams)
+        ops.reorder_states(caches, torch.arange(n, device="cuda").repeat_interleave(width).view(1, rows), length=n_prompt)
+        history[:, 0] = tokens.view(-1)
+        lengths, ended = torch.ones_like(tokens), None if eos is None else tokens == eos
+        for step in range(1, max_new_tokens):
+            if eos is not None and step % 8 == 0 and bool(ended.all()):   # (the only look from the host)
+                break
+            past = n_prompt + step - 1
+            logits = logits_of(tokens, rows, 1, past)
+            scores, beams, tokens = ops.beam_select(logits.view(n, width, -1), scores, width, ended=ended, pad=eos or 0)
+            ops.reorder_states(caches + [history], beams, length=past + 1)
+            history[:, step] = tokens.view(-1)
+            lengths = lengths.gather(1, beams) + 1
+            if eos is not None:
+                was = ended.gather(1, beams)
+                lengths, ended = lengths - was.long(), was | (tokens == eos)
+        abi.device_status()
+        found = []
+        out = (history.view(n, width, -1).cpu().numpy(), scores.cpu().numpy(), lengths.cpu().numpy(),
+               np.zeros((n, width), bool) if ended is None else ended.cpu().numpy())
+        for ids, score, length, over in zip(*out):
+            order = sorted(range(width), key=lambda w: -score[w] / float(length[w]) ** length_penalty)
+            found.append([([int(t) for t in ids[w, :length[w] - over[w]]], float(score[w])) for w in order])
+        return found[0] if single else found
 
     def _copy_stream(self):
         torch = abi.require_cuda()

@@ -90,3 +90,10 @@ def test_the_oracles_levels_are_the_nearest():
     assert [(b, t) for b, t in zip(got[1][0], got[2][0])] == [(w, v) for _, w, v in best]
     assert np.allclose(got[0][0], [c[0] for c in best])
     assert np.array_equal(beam_np.reorder(np.arange(6), np.array([[2, 2, 0], [1, 5, -1]])), [2, 2, 0, 4, 4, 5])
+
+
+def test_beams_are_searched_behind_one_prompt():
+    from rotor_b200.__main__ import main
+    for args in (["--prompt", "1", "--prompt", "2"], ["--prompt", "1", "--sampling", "top-k"]):
+        with pytest.raises(SystemExit):
+            main(["generate", "--model", "nowhere", "--beams", "2"] + args)
