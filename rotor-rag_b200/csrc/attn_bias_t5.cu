@@ -20,12 +20,8 @@
 // in turn): 8 x 2048 positions of 20 heads of 128 over 5 KV heads in chunks of 1024, with divisions and an arrival a thread / so:
 // 248 / 231 us; 16 heads with 64 shared key columns 293 / 270.  Bound by the chain of a row tile (an item of one key tile takes 7 us,
 // every further tile 1.5, of which the tensor cores work 0.6); a CTA per SM that walks the items was no faster (253).
-// Prompts over a 4-bit cache bring their keys and values as dense rows made from it, bf16 or (template parameter HALF) float16; operands,
-// weights and outputs are of that type then.
 // Waits are bounded; a wait that runs out records a code in the library status word, the CTA stops
 // issuing work, frees its tensor memory and returns.  No multicast, this GPU's memory only.
-#include <cuda_fp16.h>
-
 #include <cstdlib>
 
 #include "decoder.cuh"
@@ -44,16 +40,14 @@ struct B5Cfg {
 };
 
 struct B5Params {
-    const __nv_bfloat16* q;          // (16-bit words of the operands' type)
+    const __nv_bfloat16* q;
     __nv_bfloat16* out;
-    size_t q_seq, q_row, q_head;     // strides of the queries' sequences, tokens and heads
     const int* past_len;
     const float* slopes;
     const float* sinks;
     const float* gate;
     unsigned* status;
     int heads, kv_heads, kd, vdim, ld_out, seq, max_seq, chunk, window, ld_gate;
-    int past_most;                   // cached lengths are taken as at most this
     int rd;                          // shared key columns of a query row, behind its kd own ones
     // key j of KV head h in sequence b: row (b row_heads + h % row_heads) row_span + j - key0 of the K and V maps, from
     // columns h kx_step and vx0 + h vx_step on; its shared columns: row b max_seq + j, from column rx on
@@ -67,17 +61,7 @@ __device__ __forceinline__ float b5_exp2(float x) {
     return y;
 }
 
-template <bool HALF>
-__device__ __forceinline__ uint32_t b5_pack(float a, float b) {
-    if constexpr (HALF) {
-        const __half2 h = __floats2half2_rn(a, b);
-        return *reinterpret_cast<const uint32_t*>(&h);
-    } else {
-        return t5_pack(a, b);
-    }
-}
-
-template <int DK, int DV, int DR, bool HALF>
+template <int DK, int DV, int DR>
 __global__ void __launch_bounds__(B5_THREADS, 1)
 attn_bias_t5_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v, const __grid_constant__ CUtensorMap tm_r,
                     const __grid_constant__ B5Params p) {
@@ -96,7 +80,7 @@ attn_bias_t5_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_const
     auto position_of = [&](int r) { return (int)((uint32_t)r * per_row >> 16); };
     const int qt = gridDim.x - 1 - blockIdx.x;  // late query tiles tend to see more keys: start them first
     const int hk = blockIdx.y, b = blockIdx.z, s0 = qt * QT;
-    const int past = min(max(__ldcg(p.past_len + b), 0), p.past_most);
+    const int past = cached_len(p.past_len, b, p.max_seq);
     volatile int* abort_flag = &s_abort;
     const int s_last = min(s0 + QT, p.seq) - 1;
     const int p0 = past + s0;
@@ -143,7 +127,7 @@ attn_bias_t5_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_const
                 const bool on = c8 < DK / 8 ? col < p.kd : col < qd;
                 qv[u] = make_uint4(0u, 0u, 0u, 0u);
                 if (sp < QT && s < p.seq && on)
-                    qv[u] = __ldg(reinterpret_cast<const uint4*>(p.q + b * p.q_seq + s * p.q_row + (hk * G + gi) * p.q_head + col));
+                    qv[u] = __ldg(reinterpret_cast<const uint4*>(p.q + (((size_t)b * p.seq + s) * p.heads + hk * G + gi) * qd + col));
             }
 #pragma unroll
             for (int u = 0; u < QN; ++u) {
@@ -161,7 +145,7 @@ attn_bias_t5_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_const
         const int half = warp >> 2, wq = warp & 3, r = wq * 32 + lane;
         const int sp = min(position_of(r), QT - 1), gi = r - position_of(r) * G;
         const int pos = past + min(s0 + sp, s_last);
-        const int lo = first_visible(pos, p.chunk, p.window), hi = min(pos, p.max_seq - 1);  // visible keys [lo, hi]
+        const int lo = first_visible(pos, p.chunk, p.window), hi = pos;  // visible keys [lo, hi]
         const float slope2 = p.slopes ? __ldg(p.slopes + hk * G + gi) * 1.4426950408889634f : 0.f;
         const uint32_t lane_base = tmem + ((uint32_t)(wq * 32) << 16);
         float m_run = -INFINITY, l_run = 0.f, alpha_prev = 1.f;
@@ -235,7 +219,7 @@ attn_bias_t5_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_const
             for (int c = 0; c < 32; ++c) {
                 const float e0 = b5_exp2(sa[2 * c] - m_sub), e1 = b5_exp2(sa[2 * c + 1] - m_sub);
                 sum += e0 + e1;
-                pk[c] = b5_pack<HALF>(e0, e1);
+                pk[c] = t5_pack(e0, e1);
             }
             t5_st32(sbuf + (uint32_t)half * 32u, pk);  // 128 bf16 weights in columns [0, 64) of the S buffer
             asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
@@ -253,7 +237,7 @@ attn_bias_t5_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_const
         l_run += s_xch[half ^ 1][r];
         if (__all_sync(0xffffffffu, ok)) {
             // rows leave through a per-warp block of the operand rings (idle: every MMA has completed)
-            float inv = l_run == 0.f ? 0.f : 1.0f / l_run;  // (no key: zeros)
+            float inv = 1.0f / l_run;
             if (p.sinks) {
                 const float sink = __ldg(p.sinks + hk * G + gi) * 1.4426950408889634f, top = fmaxf(m_run, sink), mine = b5_exp2(m_run - top);
                 inv = mine / (l_run * mine + b5_exp2(sink - top));
@@ -269,12 +253,12 @@ attn_bias_t5_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_const
             if constexpr (DV == 128) {
                 uint32_t v[32];
 #pragma unroll
-                for (int i = 0; i < 32; ++i) v[i] = b5_pack<HALF>(o[2 * i] * inv, o[2 * i + 1] * inv);
+                for (int i = 0; i < 32; ++i) v[i] = t5_pack(o[2 * i] * inv, o[2 * i + 1] * inv);
                 t5_store_rows_to(blk, v, lane, dst_of);
             } else {
                 uint32_t v[16];
 #pragma unroll
-                for (int i = 0; i < 16; ++i) v[i] = b5_pack<HALF>(o[2 * i] * inv, o[2 * i + 1] * inv);
+                for (int i = 0; i < 16; ++i) v[i] = t5_pack(o[2 * i] * inv, o[2 * i + 1] * inv);
                 t5_store_half_rows_to(blk, v, lane, dst_of);
             }
         }
@@ -306,8 +290,7 @@ attn_bias_t5_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_const
         }
     } else {
         if (elect_lane()) {
-            constexpr uint32_t idesc_s = HALF ? t5_idesc_f16(128, B5_BN) : t5_idesc_bf16(128, B5_BN);
-            constexpr uint32_t idesc_o = HALF ? t5_idesc_f16(128, DV, true) : t5_idesc_bf16(128, DV, true);
+            constexpr uint32_t idesc_s = t5_idesc_bf16(128, B5_BN), idesc_o = t5_idesc_bf16(128, DV, true);
             const uint64_t dq = t5_desc(qbase);
             auto issue_s = [&](int j) {
                 const uint64_t dk = t5_desc(kring + (uint32_t)(j & 1) * C::K_BYTES);
@@ -375,19 +358,19 @@ bool bias_attn_t5_supported(const BiasAttn& p, int rows) {
            G <= B5_BM && p.ld_out % 8 == 0 && ((uintptr_t)p.out & 15) == 0 && s.kv_heads <= 65535 && rows / p.cache.seq <= 65535;
 }
 
-template <int DK, int DV, int DR, bool HALF = false>
+template <int DK, int DV, int DR>
 static int b5_go(const CUtensorMap& tk, const CUtensorMap& tv, const CUtensorMap& tr, B5Params& a, int batch, cudaStream_t st) {
     using C = B5Cfg<DK, DV, DR>;
     static PerDevice<bool> once;
     if (!once.here()) {
-        RB_CUDA(cudaFuncSetAttribute(attn_bias_t5_kernel<DK, DV, DR, HALF>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM));
+        RB_CUDA(cudaFuncSetAttribute(attn_bias_t5_kernel<DK, DV, DR>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM));
         once.here() = true;
     }
     a.status = library_status_word();
     if (!a.status) return ROTOR_B200_ERR_CUDA;
     const int QT = B5_BM / (a.heads / a.kv_heads);
     dim3 grid((a.seq + QT - 1) / QT, a.kv_heads, batch);
-    attn_bias_t5_kernel<DK, DV, DR, HALF><<<grid, B5_THREADS, C::SMEM, st>>>(tk, tv, tr, a);
+    attn_bias_t5_kernel<DK, DV, DR><<<grid, B5_THREADS, C::SMEM, st>>>(tk, tv, tr, a);
     return launch_status();
 }
 
@@ -409,10 +392,6 @@ int launch_bias_attn_t5(const BiasAttn& p, int rows, cudaStream_t st) {
     a.heads = s.heads;
     a.kv_heads = s.kv_heads;
     a.kd = s.kd;
-    a.q_head = s.kd;
-    a.q_row = (size_t)s.heads * s.kd;
-    a.q_seq = a.q_row * p.cache.seq;
-    a.past_most = p.cache.max_seq - 1;
     a.vdim = s.vdim;
     a.ld_out = p.ld_out;
     a.seq = p.cache.seq;
@@ -425,40 +404,6 @@ int launch_bias_attn_t5(const BiasAttn& p, int rows, cudaStream_t st) {
     const bool k64 = p.s.dim <= 64, v64 = p.s.vdim <= 64;
     if (k64) return v64 ? b5_go<64, 64, 0>(tk, tv, tk, a, batch, st) : b5_go<64, 128, 0>(tk, tv, tk, a, batch, st);
     return v64 ? b5_go<128, 64, 0>(tk, tv, tk, a, batch, st) : b5_go<128, 128, 0>(tk, tv, tk, a, batch, st);
-}
-
-bool prompt_attn_supported(int batch, int heads, int kv_heads, int dim, int span) {
-    static const bool off = getenv("ROTOR_B200_NO_TCGEN05") != nullptr;
-    return !off && dim <= 128 && heads / kv_heads <= B5_BM && batch <= 65535 && kv_heads <= 65535 &&
-           (size_t)batch * kv_heads * span <= 0x7fffffffu;
-}
-
-int launch_prompt_attn(const PromptAttn& p, cudaStream_t st) {
-    if (!prompt_attn_supported(p.batch, p.heads, p.kv_heads, p.dim, p.span)) return ROTOR_B200_ERR_SHAPE;
-    const size_t rows = (size_t)p.batch * p.kv_heads * p.span;
-    CUtensorMap tk, tv;
-    if (!t5_map_bf16(&tk, p.k, rows, p.dim, p.dim, B5_BN) || !t5_map_bf16(&tv, p.v, rows, p.dim, p.dim, B5_BN)) return ROTOR_B200_ERR_CUDA;
-    B5Params a = {};
-    a.q = static_cast<const __nv_bfloat16*>(p.q);
-    a.out = static_cast<__nv_bfloat16*>(p.out);
-    a.q_seq = p.q_seq;
-    a.q_row = p.q_row;
-    a.q_head = p.q_head;
-    a.past_len = p.past_len;
-    a.past_most = p.max_seq;
-    a.sinks = p.sinks;
-    a.heads = p.heads;
-    a.kv_heads = p.kv_heads;
-    a.kd = a.vdim = p.dim;
-    a.ld_out = p.heads * p.dim;
-    a.seq = p.seq;
-    a.max_seq = p.max_seq;
-    a.window = p.window;
-    a.row_heads = p.kv_heads;
-    a.row_span = p.span;
-    a.scale2 = p.scale * 1.4426950408889634f;
-    if (p.half) return p.dim <= 64 ? b5_go<64, 64, 0, true>(tk, tv, tk, a, p.batch, st) : b5_go<128, 128, 0, true>(tk, tv, tk, a, p.batch, st);
-    return p.dim <= 64 ? b5_go<64, 64, 0>(tk, tv, tk, a, p.batch, st) : b5_go<128, 128, 0>(tk, tv, tk, a, p.batch, st);
 }
 
 bool expanded_attn_supported(const LatentShape& s, int seq) {
@@ -486,10 +431,6 @@ int launch_expanded_attn(const ExpandedAttn& p, int batch, cudaStream_t st) {
     a.heads = a.kv_heads = s.heads;
     a.kd = s.dp;
     a.rd = s.rp;
-    a.q_head = s.dp + s.rp;
-    a.q_row = (size_t)s.heads * a.q_head;
-    a.q_seq = a.q_row * p.cache.seq;
-    a.past_most = p.cache.max_seq - 1;
     a.vdim = vp;
     a.ld_out = p.ld_out;
     a.seq = p.cache.seq;

@@ -206,7 +206,7 @@ struct Cache4Load {
     uint32_t units;  // kv_heads * quads * dim / 8
     FastDiv per_row, quads;
     // rows for a prompt
-    int seq, window;
+    int seq, window, negate;
     Past past;
     int* past_out;
 };
@@ -256,6 +256,7 @@ __global__ void __launch_bounds__(C4_THREADS) cache4_load_kernel(const __grid_co
             }
         }
     }
+    const float sign = PROMPT && part == 0 && p.negate ? -1.f : 1.f;
     T* dst = static_cast<T*>(p.dst[part]) + (((size_t)b * p.c.kv_heads + h) * p.span) * p.c.dim + c8 * 8;
 #pragma unroll
     for (int k = 0; k < 4; ++k) {
@@ -266,7 +267,7 @@ __global__ void __launch_bounds__(C4_THREADS) cache4_load_kernel(const __grid_co
 #pragma unroll
         for (int n = 0; n < 8; ++n) {
             x[n] = fmaf((float)(word[k] >> (4 * n) & 15u), s[k], m[k]);
-            if (PROMPT) x[n] = there ? fminf(x[n], C4_MOST) : 0.f;  // (m + 15 s may lie a rounding above the largest float16)
+            if (PROMPT) x[n] = there ? sign * fminf(x[n], C4_MOST) : 0.f;  // (m + 15 s may lie a rounding above the largest float16)
         }
         store8(dst + (size_t)(pos - p.begin) * p.c.dim, x);
     }
@@ -313,6 +314,7 @@ int launch_cache4_expand(const Cache4Expand& r, cudaStream_t st) {
     p.span = r.span;
     p.seq = r.seq;
     p.window = r.window;
+    p.negate = r.negate;
     p.past = r.past;
     p.past_out = r.past_out;
     if (const int e = load_units(p)) return e;

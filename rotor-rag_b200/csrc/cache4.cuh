@@ -134,14 +134,29 @@ int cache4_view(const rotor_b200_cache4* c, Cache4View& v);  // checks the descr
 
 
 // The first `span` positions of every sequence and head as dense rows [batch][kv_heads][span][dim], bf16 or float16, as the prompt attention
-// of `seq` tokens reads them: zeros behind a sequence's last position, nothing where no query looks.  past goes to past_out as well.
+// of `seq` tokens reads them: zeros behind a sequence's last position, nothing where no query looks, keys times -1 with `negate`.  past goes to past_out too.
 struct Cache4Expand {
     Cache4View c;
     void *k, *v;
-    int half, span, seq, window;
+    int half, span, seq, window, negate;
     Past past;
     int* past_out;
 };
 int launch_cache4_expand(const Cache4Expand& r, cudaStream_t st);
+
+// Attention of prompts over those rows.  Sequence b holds past_len[b] positions (at most max_seq) before its tokens; positions from max_seq
+// on do not exist.  Rows up to 127 behind a sequence's last one are read and multiplied by zero: they have to hold numbers.  The keys hold
+// the scale's sign.  No stride of an extent above one is zero.
+struct PromptAttn {
+    const void *q, *k, *v;
+    size_t q_seq, q_row, q_head;  // strides in elements; rows begin at multiples of 16 bytes
+    const int* past_len;
+    const float* sinks;           // [heads], or null
+    void* out;                    // [batch][seq][heads][dim]
+    int half, batch, seq, heads, kv_heads, dim, span, max_seq, window;
+    float scale;
+};
+bool prompt_attn_supported(int batch, int heads, int kv_heads, int dim, int span);
+int launch_prompt_attn(const PromptAttn& p, cudaStream_t st);
 
 }  // namespace rb

@@ -684,7 +684,7 @@ struct Attend4Plan {
 // Measured here / as prompts, 16-bit types, heads of 128: 16 tokens of 4 sequences behind 2000 positions, 20/5 heads, 16.5 / 37 us;
 // 64 tokens 47 / 40; 16 tokens behind 16000 positions, 64/8 heads, 51 / 213; 64 tokens 231 / 215; 64 tokens of 32 sequences behind 1000
 // positions, 32/8 heads, 296 / 120.
-static Attend4Plan attend4_plan(const Cache4View& c, int dtype, int heads, int seq, int longest, int window, bool wide, bool ragged) {
+static Attend4Plan attend4_plan(const Cache4View& c, int dtype, int heads, int seq, int longest, int window, bool boxes, bool ragged) {
     Attend4Plan a = {};
     const int group = heads / c.kv_heads, rows = seq * group, ng = c.dim / C4_GROUP, sms = fused_sm_count();
     const int held = (int)((long long)longest + seq < c.max_seq ? longest + seq : c.max_seq);
@@ -710,7 +710,7 @@ static Attend4Plan attend4_plan(const Cache4View& c, int dtype, int heads, int s
 
     a.span = held;
     a.dense_bytes = round_up((size_t)c.batch * c.kv_heads * a.span * c.dim * 2, 256);
-    if (wide && dtype != ROTOR_B200_F32 && rows > 16 && prompt_attn_supported(c.batch, heads, c.kv_heads, c.dim, a.span) &&
+    if (boxes && dtype != ROTOR_B200_F32 && rows > 16 && prompt_attn_supported(c.batch, heads, c.kv_heads, c.dim, a.span) &&
         (uint64_t)c.kv_heads * a.span * (c.dim / 8) <= 0x7fffff00u) {
         const double most = (reach + 127) / 128, mean = most - 0.5 * (seq < reach ? seq : reach) / 128;  // tiles of keys
         const double dense = 3.0 + (double)c.batch * c.kv_heads * reach * c.dim * 5.25 * 1e-6 / 5.0;
@@ -781,7 +781,9 @@ int rotor_b200_cache4_attend(const rotor_b200_cache4* cache, const void* q, int 
     RB_REQUIRE(s[0] >= 0 && s[1] >= 0 && s[2] >= 0 && (uintptr_t)q % size == 0 && (((uintptr_t)out | (uintptr_t)workspace) & 15) == 0);
     a.wide = (((uintptr_t)q | (uintptr_t)((s[0] | s[1] | s[2]) * size)) & 15) == 0;
     a.past = Past{past_len, past, longest < a.c.max_seq ? longest : a.c.max_seq};
-    const Attend4Plan plan = attend4_plan(a.c, dtype, heads, seq, past_len ? longest : past, window, a.wide, past_len != nullptr);
+    // (the prompt kernel copies whole boxes of queries: rows that lie apart)
+    const bool boxes = a.wide && (s[0] > 0 || a.c.batch == 1) && (s[1] > 0 || seq == 1) && (s[2] > 0 || heads == 1);
+    const Attend4Plan plan = attend4_plan(a.c, dtype, heads, seq, past_len ? longest : past, window, boxes, past_len != nullptr);
     if (plan.bytes > workspace_bytes || (plan.bytes && !workspace)) return ROTOR_B200_ERR_WORKSPACE;
     const cudaStream_t st = as_stream(stream);
     if (plan.prompt) {
@@ -793,6 +795,7 @@ int rotor_b200_cache4_attend(const rotor_b200_cache4* cache, const void* q, int 
         x.span = plan.span;
         x.seq = seq;
         x.window = window;
+        x.negate = scale < 0.f;
         x.past = a.past;
         x.past_out = reinterpret_cast<int*>(static_cast<char*>(workspace) + 2 * plan.dense_bytes);
         if (const int e = launch_cache4_expand(x, st)) return e;

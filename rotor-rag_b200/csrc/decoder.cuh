@@ -188,21 +188,6 @@ int launch_bias_attn_rows(const BiasAttn& p, int rows, cudaStream_t st);
 bool bias_attn_t5_supported(const BiasAttn& p, int rows);
 int launch_bias_attn_t5(const BiasAttn& p, int rows, cudaStream_t st);
 
-// Causal attention of `seq` tokens a sequence on the tensor cores over dense rows k, v [batch][kv_heads][span][dim], all of one 16-bit type
-// (bf16, or float16 with `half`).  Sequence b holds past_len[b] positions (at most max_seq) before its tokens; positions from max_seq on do
-// not exist.  Rows up to 127 behind a sequence's last one are read and multiplied by zero: they have to hold numbers.
-struct PromptAttn {
-    const void *q, *k, *v;
-    size_t q_seq, q_row, q_head;  // strides in elements; rows begin at multiples of 16 bytes
-    const int* past_len;
-    const float* sinks;           // [heads], or null
-    void* out;                    // [batch][seq][heads][dim]
-    int half, batch, seq, heads, kv_heads, dim, span, max_seq, window;
-    float scale;
-};
-bool prompt_attn_supported(int batch, int heads, int kv_heads, int dim, int span);
-int launch_prompt_attn(const PromptAttn& p, cudaStream_t st);
-
 // Latent attention.  A position's cache row is [latent, rank rounded up to 16 | rotated key part, rot_dim rounded
 // up to 16], pads zero; a head's query row is [dim rounded up to 8 | rot rounded up to 16].
 //   absorbed: the queries are taken into the latent space (W_uk^T q), scores and values come from the cache rows

@@ -192,6 +192,23 @@ def test_portions_and_prompts(torch, seq, heads, kv, past, dtype):
     attend_case(torch, seq + 1, 1, seq, heads, kv, 128, past, dtype=dtype, window=21)
 
 
+@pytest.mark.parametrize("dtype", ["bfloat16", "float16"])
+@pytest.mark.parametrize("seq,heads,kv,dim,past,kw", [
+    (300, 20, 5, 128, 0, {}), (257, 12, 4, 64, 200, {}), (300, 6, 6, 96, [0, 77], {}), (300, 8, 2, 32, 3, {}), (200, 64, 8, 128, 100, {}),
+    (300, 8, 1, 128, [300, 5], {"window": 99}), (290, 9, 3, 64, [400, 0], {"window": 130, "sinks": True}), (300, 8, 2, 128, 0, {"sinks": True}),
+    (520, 7, 1, 128, 0, {"scale": -0.07}), (256, 16, 4, 128, 0, {"scale": 0.0}), (260, 8, 2, 128, 900, {"scale": 1.5})])
+def test_prompts_on_the_prompt_kernel(torch, seq, heads, kv, dim, past, kw, dtype):
+    """Sizes that are worth dense rows: the workspace holds them."""
+    from rotor_b200 import abi, ops
+    from rotor_b200.cache4 import Cache4
+    batch = 2
+    high = past if isinstance(past, int) else max(past)
+    need = abi.lib.rotor_b200_cache4_attend_workspace_bytes(Cache4(batch, kv, high + seq, dim)._ref, ops.type_code(getattr(torch, dtype)), heads, seq, high,
+                                                            kw.get("window", 0))
+    # assert need >= 4 * batch * kv * (high + seq) * dim
+    attend_case(torch, seq + heads, batch, seq, heads, kv, dim, past, dtype=dtype, lengths=None if isinstance(past, int) else high, **kw)
+
+
 @pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("window", [1, 2, 16, 17, 100, 5000])
 def test_windows_and_sinks(torch, window, dtype):
