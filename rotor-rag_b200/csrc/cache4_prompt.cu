@@ -6,12 +6,20 @@
 // output blocks, 512 columns in all:
 //   S_w = Q_w K^T : Q_w and K tile by TMA
 //   O_w += P_w V  : P_w from tensor memory (written over S_w), V tile by TMA as it lies in the dense rows
-// A thread of warps 0 .. 7 owns a row of its block: it reads its 128 scores, masks them where the tile reaches over what the row sees, and
-// writes 128 weights back; no row is exchanged between threads.  While one block's scores become weights, the tensor cores work for the
-// other, and while a block's outputs are read, its next queries arrive.  Outputs stay in tensor memory: the reference that weights are
-// relative to moves, and the sums are scaled, only where a row's maximum has grown by more than 2^8 (weights are at most that, the sum of
-// weights is float32).  Warp 8: TMA; warp 9: MMA issue; the scores of a tile overwrite weights that an MMA issued before reads, in the order
-// of issue.  The eight warps take the registers that the other four give back (232 and 40 of 168 each at launch).
+// A thread of warps 4 .. 11 owns a row of its block: it reads its 128 scores, masks them where the tile reaches over what the row sees, and
+// writes 128 weights back, half of them at a time, so that the sums over the first half start while the second is made; no row is exchanged
+// between threads.  While one block's scores become weights, the tensor cores work for the other, and while a block's outputs are read, its
+// next queries arrive.  Outputs stay in tensor memory: the reference that weights are relative to moves, and the sums are scaled, only where a
+// row's maximum has grown by more than 2^8 (weights are at most that, the sum of weights is float32).  Warp 0: TMA; warp 1: MMA issue, all of
+// one thread and executed in the order of issue: the scores of a tile overwrite weights that an MMA issued before reads.  The eight warps take
+// registers that the other four give back (216 and 72 of 168 each at launch; with 40 for the four the thread that issues spilled, 2% of the
+// time).
+// Bound: a tile of both blocks takes the tensor cores 2048 clocks and 3600 in all.  The chain of a block is weights (1900 clocks for 128 x 128:
+// 550 instructions a warp, and the other block's warps share the schedulers) -> sums -> next scores (1024 clocks of MMA, some 600 of barriers:
+// a barrier operation queues behind the special function unit's, 250 clocks).  Measured, bf16, 32 query and 8 KV heads of 128, causal, with the
+// dense rows made first: 8192 tokens of one sequence 508 us (1.08 PFLOP/s), 8 x 2048 tokens of 20 and 5 heads 192 us (0.90).  Tried and
+// slower: weights in one piece (3%); half or a quarter of the exponentials by polynomials in the FMA pipe (10%, 0%); steps of 64 keys with two
+// score blocks in flight for each block (30%: twice the barriers); items in the same order for every round of CTAs (8%).
 // Waits are bounded; a wait that runs out records a code in the library status word, the CTA stops issuing work, frees its tensor memory
 // and returns.  No multicast, this GPU's memory only.
 #include <cstdlib>
@@ -22,12 +30,13 @@
 namespace rb {
 
 constexpr int P4_ROWS = 128, P4_KEYS = 128, P4_THREADS = 384;
-constexpr int P4_SOFT_REGS = 232, P4_OTHER_REGS = 40, P4_REGS = 168;  // 2 x 128 x 232 + 128 x 40 = 384 x 168
+constexpr int P4_SOFT_REGS = 216, P4_OTHER_REGS = 72, P4_REGS = 168;  // 2 x 128 x 216 + 128 x 72 = 384 x 168
 constexpr float P4_SLACK = 8.f;
 
 template <int DK>
 struct P4Cfg {
-    static constexpr int TILE = P4_KEYS * DK * 2, SMEM = 6 * TILE + 1024;  // two query blocks, two tiles of keys and two of values
+    // two query blocks, and a ring of tiles that keys and values take in turn: of 128 columns as many as fit
+    static constexpr int TILE = P4_KEYS * DK * 2, SLOTS = DK == 128 ? 5 : 8, SMEM = (2 + SLOTS) * TILE + 1024;
 };
 
 struct P4Params {
@@ -52,7 +61,13 @@ __device__ __forceinline__ uint32_t p4_pack(float a, float b) {
     return HALF ? pack_half(a, b) : t5_pack(a, b);
 }
 
-// Item i of a call: the blocks of late tokens, which see more keys, come first.
+// Item i of a call: the blocks of late tokens, which see more keys, come first.  CTAs take a round of items in one order and the next round
+// in the other, so that none gets the longest of every round.
+__device__ __forceinline__ int p4_item(int round) {
+    const int first = round * (int)gridDim.x;
+    return round & 1 ? first + (int)gridDim.x - 1 - (int)blockIdx.x : first + (int)blockIdx.x;
+}
+
 struct P4Item {
     int b, hk, s0, s_last, past, kb0, ntiles;
     __device__ __forceinline__ P4Item(const P4Params& p, int i) {
@@ -75,31 +90,34 @@ cache4_prompt_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_cons
                      const __grid_constant__ P4Params p) {
     using C = P4Cfg<DK>;
     extern __shared__ unsigned char p4_raw[];
-    __shared__ __align__(8) unsigned long long s_kfull[2], s_kempty[2], s_vfull[2], s_vempty[2], s_sfull[2], s_pfull[2], s_done[2], s_qfull[2],
-        s_qempty[2];
+    __shared__ __align__(8) unsigned long long s_full[C::SLOTS], s_empty[C::SLOTS], s_sfull[2], s_pfull[2][2], s_done[2], s_qfull[2], s_qempty[2];
     __shared__ uint32_t s_tmem;
     __shared__ int s_abort;
-    const uint32_t qbase = (smem_u32(p4_raw) + 1023u) & ~1023u, kring = qbase + 2 * C::TILE, vring = kring + 2 * C::TILE;
+    const uint32_t qbase = (smem_u32(p4_raw) + 1023u) & ~1023u, ring = qbase + 2 * C::TILE;
+    // keys of the CTA's tile t are load 2 t, values load 2 t + 1
+    auto slot_of = [](uint32_t load) { return load % C::SLOTS; };
+    auto parity_of = [](uint32_t load) { return load / C::SLOTS & 1u; };
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int G = p.heads / p.kv_heads, QT = P4_ROWS / G;  // tokens of a block
     volatile int* abort_flag = &s_abort;
 
     if (threadIdx.x == 0) {
         s_abort = 0;
+        for (int s = 0; s < C::SLOTS; ++s) {
+            t5_bar_init(smem_u32(&s_full[s]), 1);
+            t5_bar_init(smem_u32(&s_empty[s]), 1);
+        }
         for (int s = 0; s < 2; ++s) {
-            t5_bar_init(smem_u32(&s_kfull[s]), 1);
-            t5_bar_init(smem_u32(&s_kempty[s]), 1);
-            t5_bar_init(smem_u32(&s_vfull[s]), 1);
-            t5_bar_init(smem_u32(&s_vempty[s]), 1);
             t5_bar_init(smem_u32(&s_sfull[s]), 1);
-            t5_bar_init(smem_u32(&s_pfull[s]), 4);
+            t5_bar_init(smem_u32(&s_pfull[s][0]), 4);
+            t5_bar_init(smem_u32(&s_pfull[s][1]), 4);
             t5_bar_init(smem_u32(&s_done[s]), 1);
             t5_bar_init(smem_u32(&s_qfull[s]), 1);
             t5_bar_init(smem_u32(&s_qempty[s]), 1);
         }
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
-    if (warp == 8) {
+    if (warp == 0) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&s_tmem)), "r"(512));
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::);
     }
@@ -108,17 +126,17 @@ cache4_prompt_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_cons
     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
     const uint32_t tmem = s_tmem;  // S_0 [0, 128)  S_1 [128, 256)  O_0 [256, 256 + DK)  O_1 [384, 384 + DK)
 
-    if (warp < 8) {
+    if (warp >= 4) {
         asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(P4_SOFT_REGS));
-        const int w = warp >> 2, r = (warp & 3) * 32 + lane;  // block and row
+        const int w = (warp >> 2) - 1, r = (warp & 3) * 32 + lane;  // block and row
         const int in_block = r / G, gi = r - in_block * G;
         const uint32_t lane_base = tmem + ((uint32_t)((warp & 3) * 32) << 16);
         const uint32_t sbuf = lane_base + (uint32_t)w * 128u, obuf = lane_base + 256u + (uint32_t)w * 128u;
         const float2 scale = make_float2(p.scale2, p.scale2);
         bool ok = true;
         uint32_t tile = 0;  // of the CTA, over its items
-        for (int item = blockIdx.x; item < p.items && ok; item += gridDim.x) {
-            const P4Item it(p, item);
+        for (int round = 0; ok && p4_item(round) < p.items; ++round) {
+            const P4Item it(p, p4_item(round));
             const int token = it.s0 + w * QT + in_block, pos = it.past + min(token, it.s_last);
             const bool real = in_block < QT && token <= it.s_last;
             const int lo = first_visible(pos, 0, p.window), hi = min(pos, p.max_seq - 1);  // visible keys [lo, hi]
@@ -179,21 +197,21 @@ cache4_prompt_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_cons
                         pk[i] = p4_pack<HALF>(e.x, e.y);
                     }
                     t5_st32(sbuf + (uint32_t)h * 32u, pk);  // 128 weights in columns [0, 64) of the scores' block
+                    asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
+                    asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+                    __syncwarp();
+                    if (lane == 0) t5_bar_arrive(smem_u32(&s_pfull[w][h]));
                 }
                 mass += (sum[0].x + sum[0].y) + (sum[1].x + sum[1].y);
-                asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
-                asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
-                __syncwarp();
-                if (lane == 0) t5_bar_arrive(smem_u32(&s_pfull[w]));
             }
             if (ok && it.ntiles > 0)
                 ok = __all_sync(0xffffffffu, t5_wait(smem_u32(&s_done[w]), (tile - 1u) & 1u, abort_flag, p.status, 0x7b000003u));
             if (!ok) break;
             asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-            float inv = mass == 0.f ? 0.f : 1.f / mass;  // (no key: zeros)
+            float inv = ref == -INFINITY && mass == mass ? 0.f : 1.f / mass;  // (no key: zeros)
             if (p.sinks && real) {
                 const float sink = __ldg(p.sinks + it.hk * G + gi) * 1.4426950408889634f, most = fmaxf(ref, sink), mine = fast_exp2(ref - most);
-                inv = mine / (mass * mine + fast_exp2(sink - most));
+                inv = ref == -INFINITY && mass == mass ? 0.f : mine / (mass * mine + fast_exp2(sink - most));
             }
             uint16_t* out = p.out + (((size_t)it.b * p.seq + (real ? token : 0)) * p.heads + it.hk * G + gi) * p.dim;
 #pragma unroll
@@ -221,11 +239,11 @@ cache4_prompt_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_cons
         }
     } else {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(P4_OTHER_REGS));
-        if (warp == 8 && elect_lane()) {
-            uint32_t tile = 0, nth = 0;  // of the CTA
+        if (warp == 0 && elect_lane()) {
+            uint32_t load = 0, nth = 0;  // of the CTA
             bool ok = true;
-            for (int item = blockIdx.x; item < p.items && ok; item += gridDim.x) {
-                const P4Item it(p, item);
+            for (int round = 0; ok && p4_item(round) < p.items; ++round) {
+                const P4Item it(p, p4_item(round));
                 if (it.ntiles == 0) continue;
                 const int row0 = (it.b * p.kv_heads + it.hk) * p.span + it.kb0;
                 auto queries = [&](int w) {
@@ -239,54 +257,50 @@ cache4_prompt_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_cons
                 };
                 ok = queries(0) && queries(1);
                 ++nth;
-                for (int j = 0; j < it.ntiles && ok; ++j, ++tile) {
-                    const uint32_t s = tile & 1u, parity = ((tile >> 1) & 1u) ^ 1u;
-                    ok = t5_wait(smem_u32(&s_kempty[s]), parity, abort_flag, p.status, 0x7b000005u);
+                for (int j = 0; j < 2 * it.ntiles && ok; ++j, ++load) {  // keys and values of a tile, in turn
+                    const uint32_t slot = slot_of(load), bar = smem_u32(&s_full[slot]);
+                    ok = t5_wait(smem_u32(&s_empty[slot]), parity_of(load) ^ 1u, abort_flag, p.status, 0x7b000005u);
                     if (!ok) break;
-                    uint32_t bar = smem_u32(&s_kfull[s]);
                     t5_bar_expect(bar, C::TILE);
 #pragma unroll
-                    for (int pn = 0; pn < DK / 64; ++pn) t5_tma_2d(kring + s * C::TILE + pn * 16384, &tm_k, pn * 64, row0 + j * P4_KEYS, bar);
-                    ok = t5_wait(smem_u32(&s_vempty[s]), parity, abort_flag, p.status, 0x7b000006u);
-                    if (!ok) break;
-                    bar = smem_u32(&s_vfull[s]);
-                    t5_bar_expect(bar, C::TILE);
-#pragma unroll
-                    for (int pn = 0; pn < DK / 64; ++pn) t5_tma_2d(vring + s * C::TILE + pn * 16384, &tm_v, pn * 64, row0 + j * P4_KEYS, bar);
+                    for (int pn = 0; pn < DK / 64; ++pn)
+                        t5_tma_2d(ring + slot * C::TILE + pn * 16384, j & 1 ? &tm_v : &tm_k, pn * 64, row0 + (j >> 1) * P4_KEYS, bar);
                 }
             }
-        } else if (warp == 9 && elect_lane()) {
+        } else if (warp == 1 && elect_lane()) {
             constexpr uint32_t idesc_s = HALF ? t5_idesc_f16(128, P4_KEYS) : t5_idesc_bf16(128, P4_KEYS);
             constexpr uint32_t idesc_o = HALF ? t5_idesc_f16(128, DK, true) : t5_idesc_bf16(128, DK, true);
             // scores of block w and the CTA's tile t; `last`: of the item, whose queries are read for the last time
             auto issue_s = [&](int w, uint32_t t, bool last) {
-                const uint64_t dq = t5_desc(qbase + w * C::TILE), dk = t5_desc(kring + (t & 1u) * C::TILE);
+                const uint64_t dq = t5_desc(qbase + w * C::TILE), dk = t5_desc(ring + slot_of(2 * t) * C::TILE);
 #pragma unroll
                 for (int k16 = 0; k16 < DK / 16; ++k16) {
                     const uint64_t off = (uint64_t)(((k16 >> 2) * 16384 + (k16 & 3) * 32) >> 4);
                     t5_mma_ss(tmem + (uint32_t)w * 128u, dq + off, dk + off, idesc_s, k16 > 0);
                 }
                 t5_commit(smem_u32(&s_sfull[w]));
-                if (w == 1) t5_commit(smem_u32(&s_kempty[t & 1u]));
+                if (w == 1) t5_commit(smem_u32(&s_empty[slot_of(2 * t)]));
                 if (last) t5_commit(smem_u32(&s_qempty[w]));
             };
-            auto issue_pv = [&](int w, uint32_t t, bool first) {
-                const uint64_t dv = t5_desc_mn(vring + (t & 1u) * C::TILE, 16384);
+            auto issue_pv = [&](int w, uint32_t t, int half, bool first) {
+                const uint64_t dv = t5_desc_mn(ring + slot_of(2 * t + 1) * C::TILE, 16384);
 #pragma unroll
-                for (int k16 = 0; k16 < P4_KEYS / 16; ++k16)
+                for (int k = 0; k < P4_KEYS / 32; ++k) {
+                    const int k16 = half * (P4_KEYS / 32) + k;
                     t5_mma_ts(tmem + 256u + (uint32_t)w * 128u, tmem + (uint32_t)w * 128u + (uint32_t)k16 * 8u, dv + (uint64_t)(k16 * 2048 >> 4), idesc_o,
                               !first || k16 > 0);
+                }
+                if (half == 0) return;
                 t5_commit(smem_u32(&s_done[w]));
-                if (w == 1) t5_commit(smem_u32(&s_vempty[t & 1u]));
+                if (w == 1) t5_commit(smem_u32(&s_empty[slot_of(2 * t + 1)]));
             };
             // The tiles of the CTA's items in a row: scores of tile t + 1 are issued behind the sums of tile t, across items too.
-            int item = blockIdx.x, left = 0;  // left: tiles of the item after the next one to score
+            int round = 0, left = 0;  // left: tiles of the item after the next one to score
             uint32_t nth = 0;                 // items begun
             auto begin = [&]() {              // the next item that has tiles
-                for (; item < p.items; item += gridDim.x) {
-                    left = P4Item(p, item).ntiles;
+                while (p4_item(round) < p.items) {
+                    left = P4Item(p, p4_item(round++)).ntiles;
                     if (left > 0) {
-                        item += gridDim.x;
                         ++nth;
                         return true;
                     }
@@ -297,13 +311,14 @@ cache4_prompt_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_cons
             bool first_s = true;              // the tile to score is its item's first
             auto score = [&](int w, uint32_t t) {
                 if (first_s && !t5_wait(smem_u32(&s_qfull[w]), (nth - 1u) & 1u, abort_flag, p.status, 0x7b000007u)) return false;
-                if (w == 0 && !t5_wait(smem_u32(&s_kfull[t & 1u]), (t >> 1) & 1u, abort_flag, p.status, 0x7b000008u)) return false;
-                asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
                 issue_s(w, t, left == 1);
                 return true;
             };
             uint32_t t = 0;
-            if (more) ok = score(0, 0) && score(1, 0);
+            auto loaded = [&](uint32_t load) {
+                return t5_wait(smem_u32(&s_full[slot_of(load)]), parity_of(load), abort_flag, p.status, 0x7b000008u);
+            };
+            if (more) ok = loaded(0) && score(0, 0) && score(1, 0);
             bool first_pv = true;             // the tile to sum is its item's first
             while (more && ok) {
                 const bool ends = left == 1;  // tile t is its item's last
@@ -316,11 +331,15 @@ cache4_prompt_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_cons
                 }
 #pragma unroll
                 for (int w = 0; w < 2; ++w) {
-                    if (ok) ok = t5_wait(smem_u32(&s_pfull[w]), t & 1u, abort_flag, p.status, 0x7b000009u);
-                    if (ok && w == 0) ok = t5_wait(smem_u32(&s_vfull[t & 1u]), (t >> 1) & 1u, abort_flag, p.status, 0x7b00000au);
+                    if (ok && w == 0) ok = loaded(2 * t + 1) && (!more || loaded(2 * t + 2));
+#pragma unroll
+                    for (int half = 0; half < 2; ++half) {
+                        if (ok) ok = t5_wait(smem_u32(&s_pfull[w][half]), t & 1u, abort_flag, p.status, 0x7b000009u);
+                        if (!ok) break;
+                        asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+                        issue_pv(w, t, half, first_pv);
+                    }
                     if (!ok) break;
-                    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-                    issue_pv(w, t, first_pv);
                     if (more) ok = score(w, t + 1);
                 }
                 first_pv = ends;
@@ -337,7 +356,7 @@ cache4_prompt_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_cons
     }
     asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
     __syncthreads();
-    if (warp == 8) {
+    if (warp == 0) {
         asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512));
     }
