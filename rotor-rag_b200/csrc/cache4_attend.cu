@@ -679,11 +679,13 @@ struct Attend4Plan {
 // For sequences that hold up to `longest` positions (each its own number of them: `ragged`).  What is fastest goes by estimates in us:
 //   here      two CTAs (R NG > 4: one) are on an SM; a CTA takes about 4 us beside its tiles (lengths and queries arrive, the warps' sums are
 //             joined), 0.7 more for a join inside a cluster and 3.5 for the join kernel; a tile of 128 columns of every warp 0.9 us
-//             (the rate of the memory), of sixteen query rows, with a CTA on an SM, 0.75
-//   prompts   dense rows at about 5 TB/s and 3 us, then a CTA per 128 query rows, 7 us and 1.5 for every 128 keys
-// Measured here / as prompts, 16-bit types, heads of 128: 16 tokens of 4 sequences behind 2000 positions, 20/5 heads, 16.5 / 37 us;
-// 64 tokens 47 / 40; 16 tokens behind 16000 positions, 64/8 heads, 51 / 213; 64 tokens 231 / 215; 64 tokens of 32 sequences behind 1000
-// positions, 32/8 heads, 296 / 120.
+//             (the rate of the memory), of sixteen query rows 1.5, with a CTA on an SM 0.75
+//   prompts   dense rows at about 5 TB/s and 3 us, then a CTA per SM, 9 us and for every 128 keys of its items (two blocks of 128 query rows)
+//             1.8, with many items on every SM 2.2 and 1 for an item
+// Measured here / as prompts, bf16, heads of 128: 16 tokens of 4 sequences behind 2000 positions, 20/5 heads, 17.5 / 43.1 us, 64 tokens
+// 49.1 / 48.2, 256 tokens 148 / 51.7; 16 tokens behind 16000 positions, 64/8 heads, 53 / 246, 64 tokens 232 / 246, 128 tokens 356 / 247;
+// 32 sequences, 32/8 heads, behind 500 positions: 16 tokens 52 / 56, 32 tokens 104 / 60, 256 tokens 942 / 155.  Heads of 64, 8 sequences, 16/4
+// heads, behind 2000 positions: 64 tokens 37 / 43, 128 tokens 64 / 44.
 static Attend4Plan attend4_plan(const Cache4View& c, int dtype, int heads, int seq, int longest, int window, bool boxes, bool ragged) {
     Attend4Plan a = {};
     const int group = heads / c.kv_heads, rows = seq * group, ng = c.dim / C4_GROUP, sms = fused_sm_count();
@@ -693,7 +695,7 @@ static Attend4Plan attend4_plan(const Cache4View& c, int dtype, int heads, int s
     const long long blocks = (long long)c.batch * c.kv_heads * ((rows + a.per_block - 1) / a.per_block), tiles = (reach + 15) / 16 + 1;
     const bool pair = ng * a.per_block <= 32;
     const long long slots = sms * (pair ? 2 : 1);
-    const double tile_us = (pair ? 0.9 : 0.75) * ng / 4;
+    const double tile_us = (!pair ? 0.75 : a.per_block == 16 ? 1.5 : 0.9) * ng / 4;
     double best = 1e30;
     auto consider = [&](long long splits) {
         if (splits < 1 || (splits - 1) * 8 >= tiles) return;
@@ -714,9 +716,10 @@ static Attend4Plan attend4_plan(const Cache4View& c, int dtype, int heads, int s
         (uint64_t)c.kv_heads * a.span * (c.dim / 8) <= 0x7fffff00u) {
         const double most = (reach + 127) / 128, mean = most - 0.5 * (seq < reach ? seq : reach) / 128;  // tiles of keys
         const double dense = 3.0 + (double)c.batch * c.kv_heads * reach * c.dim * 5.25 * 1e-6 / 5.0;
-        const double ctas = (double)c.batch * c.kv_heads * ((seq + 128 / group - 1) / (128 / group));
-        const double one = 7.0 + 1.5 * most, all = ctas / sms * (7.0 + 1.5 * mean);
-        a.prompt = dense + (one > all ? one : all) < best;
+        const int tokens = 2 * (128 / group);
+        const long long items = (long long)c.batch * c.kv_heads * ((seq + tokens - 1) / tokens);
+        const double one = 1.8 * most, all = (double)((items + sms - 1) / sms) * (1.0 + 2.2 * mean);
+        a.prompt = dense + 9.0 + (one > all ? one : all) < best;
     }
     if (a.prompt) {
         a.bytes = 2 * a.dense_bytes + (size_t)c.batch * sizeof(int);

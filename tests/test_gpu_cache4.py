@@ -201,11 +201,12 @@ def test_prompts_on_the_prompt_kernel(torch, seq, heads, kv, dim, past, kw, dtyp
     """Sizes that are worth dense rows: the workspace holds them."""
     from rotor_b200 import abi, ops
     from rotor_b200.cache4 import Cache4
-    batch = 2
+    batch = 8
+    past = past if isinstance(past, int) else past * 4
     high = past if isinstance(past, int) else max(past)
     need = abi.lib.rotor_b200_cache4_attend_workspace_bytes(Cache4(batch, kv, high + seq, dim)._ref, ops.type_code(getattr(torch, dtype)), heads, seq, high,
                                                             kw.get("window", 0))
-    # assert need >= 4 * batch * kv * (high + seq) * dim
+    assert need >= 4 * batch * kv * (high + seq) * dim
     attend_case(torch, seq + heads, batch, seq, heads, kv, dim, past, dtype=dtype, lengths=None if isinstance(past, int) else high, **kw)
 
 
