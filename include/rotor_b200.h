@@ -426,7 +426,7 @@ int rotor_b200_sample(const float* logits, int rows, int vocab, int mode, int to
  *    [groups][count].  workspace: 16-byte aligned, contents of no matter, rotor_b200_beam_select_workspace_bytes bytes; calls that use
  *    none (few logits) take NULL, and the others return ERR_WORKSPACE before anything is launched.
  *  reorder_states: row b * width + w of every state becomes what row b * width + beams[b][w] was, in place; rows whose beam is
- *    their own, or no index of the group, stay.  `states` is a HOST array; width <= 32. */
+ *    their own, or no index of the group, stay.  `states` is a HOST array, whose memory does not overlap; width <= 32. */
 #define ROTOR_B200_F32 0
 #define ROTOR_B200_BF16 1
 #define ROTOR_B200_F16 2
@@ -462,7 +462,7 @@ int rotor_b200_reorder_states(const rotor_b200_state* states, int n, const int64
  *    with window > 0 those with (own - j) < window.  Softmax of scale * q . k, whose denominator holds exp(sinks[head]) as well
  *    (sinks float32 [heads] or NULL); query head h reads KV head h / (heads / kv_heads).  out: `dtype` [batch][seq][heads][dim],
  *    16-byte aligned.  A query that sees no position gives zeros.  `longest`: with past_len, the most that a sequence holds, by which the
- *    work is divided; longer lengths are taken as it.  Without, not read.  workspace: 16-byte aligned, contents of no
+ *    work is divided; longer lengths are taken as it.  Without, of no effect.  workspace: 16-byte aligned, contents of no
  *    matter, rotor_b200_cache4_attend_workspace_bytes bytes (given `longest` = past where past_len is NULL; 0: not supported); calls
  *    that use none, steps of a few tokens over caches that are not long, take NULL, and the others return ERR_WORKSPACE before
  *    anything is launched. */

@@ -33,6 +33,9 @@ constexpr float A4_LOW = -1e30f;  // a shift that any score is above
 constexpr int A4_JOIN = 256;      // threads of the join
 constexpr int A4_SORTED = 128;    // most sequences that are taken by their length
 constexpr int A4_CLUSTER = 8;     // most splits that are joined inside a cluster
+// Dense keys (and values) of a prompt at a time, unless one sequence has more: the rows take 3.2 times the cache's memory, and sequences after
+// one another keep the workspace at 1 GiB.  (That much is 0.4 ms of writing alone: a launch more does not show.)
+constexpr size_t A4_DENSE = (size_t)1 << 29;
 
 struct Attend4 {
     Cache4View c;
@@ -670,7 +673,7 @@ __global__ void __launch_bounds__(A4_JOIN) attend4_join_kernel(const __grid_cons
 
 struct Attend4Plan {
     bool prompt;             // the cache's rows are made dense (bf16 or float16) in the workspace, for the prompt kernel
-    int span;                // prompt: dense rows of a head
+    int span, chunk;         // prompt: dense rows of a head, sequences at a time
     size_t dense_bytes;      // of the keys, and of the values
     int splits, per_block, by_length;  // else: CTAs that share a row's positions, query rows of a block, longest sequences first
     size_t bytes;            // of workspace
@@ -711,8 +714,10 @@ static Attend4Plan attend4_plan(const Cache4View& c, int dtype, int heads, int s
     consider(slots / blocks > A4_CLUSTER ? (tiles + 7) / 8 : 0);
 
     a.span = held;
-    a.dense_bytes = round_up((size_t)c.batch * c.kv_heads * a.span * c.dim * 2, 256);
-    if (boxes && dtype != ROTOR_B200_F32 && rows > 16 && prompt_attn_supported(c.batch, heads, c.kv_heads, c.dim, a.span) &&
+    const size_t each = (size_t)c.kv_heads * a.span * c.dim * 2;
+    a.chunk = (int)(each * c.batch <= A4_DENSE ? c.batch : each < A4_DENSE ? A4_DENSE / each : 1);
+    a.dense_bytes = round_up(each * a.chunk, 256);
+    if (boxes && dtype != ROTOR_B200_F32 && rows > 16 && prompt_attn_supported(a.chunk, heads, c.kv_heads, c.dim, a.span) &&
         (uint64_t)c.kv_heads * a.span * (c.dim / 8) <= 0x7fffff00u) {
         const double most = (reach + 127) / 128, mean = most - 0.5 * (seq < reach ? seq : reach) / 128;  // tiles of keys
         const double dense = 3.0 + (double)c.batch * c.kv_heads * reach * c.dim * 5.25 * 1e-6 / 5.0;
@@ -722,7 +727,7 @@ static Attend4Plan attend4_plan(const Cache4View& c, int dtype, int heads, int s
         a.prompt = dense + 9.0 + (one > all ? one : all) < best;
     }
     if (a.prompt) {
-        a.bytes = 2 * a.dense_bytes + (size_t)c.batch * sizeof(int);
+        a.bytes = 2 * a.dense_bytes + (size_t)a.chunk * sizeof(int);
         return a;
     }
     a.by_length = ragged && c.batch <= A4_SORTED && blocks * a.splits > slots;
@@ -749,6 +754,18 @@ static int attend4_pick(const Attend4& a, const Attend4Plan& plan, cudaStream_t 
     const bool f32 = a.dtype == ROTOR_B200_F32;
     if (plan.per_block == 16) return f32 ? attend4_go<NG, 2, 2, 8>(a, st) : attend4_go<NG, 2, 1, 8>(a, st);
     return f32 ? attend4_go<NG, 1, 2, 8>(a, st) : attend4_go<NG, 1, 1, 8>(a, st);
+}
+
+// Sequences b .. b + n - 1, or as many as there are.
+static Cache4View cache4_part(Cache4View c, int b, int n) {
+    const size_t rows = (size_t)b * c.kv_heads * c.max_seq;
+    for (int i = 0; i < 2; ++i) {
+        c.codes[i] += rows * (c.dim / 2);
+        c.step[i] += rows * (c.dim / C4_GROUP);
+        c.least[i] += rows * (c.dim / C4_GROUP);
+    }
+    c.batch = n < c.batch - b ? n : c.batch - b;
+    return c;
 }
 
 static int attend4_check(const rotor_b200_cache4* cache, Cache4View& c, int dtype, int heads, int seq, int longest, int window) {
@@ -791,7 +808,6 @@ int rotor_b200_cache4_attend(const rotor_b200_cache4* cache, const void* q, int 
     const cudaStream_t st = as_stream(stream);
     if (plan.prompt) {
         Cache4Expand x;
-        x.c = a.c;
         x.k = workspace;
         x.v = static_cast<char*>(workspace) + plan.dense_bytes;
         x.half = dtype == ROTOR_B200_F16;
@@ -799,11 +815,8 @@ int rotor_b200_cache4_attend(const rotor_b200_cache4* cache, const void* q, int 
         x.seq = seq;
         x.window = window;
         x.negate = scale < 0.f;
-        x.past = a.past;
         x.past_out = reinterpret_cast<int*>(static_cast<char*>(workspace) + 2 * plan.dense_bytes);
-        if (const int e = launch_cache4_expand(x, st)) return e;
         PromptAttn p;
-        p.q = q;
         p.k = x.k;
         p.v = x.v;
         p.q_seq = s[0];
@@ -811,9 +824,7 @@ int rotor_b200_cache4_attend(const rotor_b200_cache4* cache, const void* q, int 
         p.q_head = s[2];
         p.past_len = x.past_out;
         p.sinks = sinks;
-        p.out = out;
         p.half = x.half;
-        p.batch = a.c.batch;
         p.seq = seq;
         p.heads = heads;
         p.kv_heads = a.c.kv_heads;
@@ -822,7 +833,16 @@ int rotor_b200_cache4_attend(const rotor_b200_cache4* cache, const void* q, int 
         p.max_seq = a.c.max_seq;
         p.window = window;
         p.scale = scale;
-        return launch_prompt_attn(p, st);
+        for (int b = 0; b < a.c.batch; b += plan.chunk) {
+            x.c = cache4_part(a.c, b, plan.chunk);
+            x.past = Past{past_len ? past_len + b : nullptr, a.past.all, a.past.most};
+            p.batch = x.c.batch;
+            p.q = static_cast<const uint16_t*>(q) + (size_t)b * s[0];
+            p.out = static_cast<uint16_t*>(out) + (size_t)b * seq * heads * a.c.dim;
+            if (const int e = launch_cache4_expand(x, st)) return e;
+            if (const int e = launch_prompt_attn(p, st)) return e;
+        }
+        return ROTOR_B200_OK;
     }
     a.q = q;
     a.qb = s[0];

@@ -13,8 +13,20 @@ static PerDevice<unsigned*> g_status_words;
 static int ensure_status() {
     unsigned*& w = g_status_words.here();
     if (w) return ROTOR_B200_OK;
-    RB_CUDA(cudaMalloc(&w, sizeof(unsigned)));
-    RB_CUDA(cudaMemset(w, 0, sizeof(unsigned)));
+    // The first call that needs the word may be captured: this thread may allocate meanwhile, and a stream of its own clears the word.
+    cudaStreamCaptureMode mode = cudaStreamCaptureModeRelaxed;
+    RB_CUDA(cudaThreadExchangeStreamCaptureMode(&mode));
+    unsigned* made = nullptr;
+    cudaStream_t own = nullptr;
+    cudaError_t e = cudaMalloc(&made, sizeof(unsigned));
+    if (e == cudaSuccess) e = cudaStreamCreateWithFlags(&own, cudaStreamNonBlocking);
+    if (e == cudaSuccess) e = cudaMemsetAsync(made, 0, sizeof(unsigned), own);
+    if (e == cudaSuccess) e = cudaStreamSynchronize(own);
+    if (own) cudaStreamDestroy(own);
+    if (e == cudaSuccess) w = made;
+    else if (made) cudaFree(made);
+    cudaThreadExchangeStreamCaptureMode(&mode);
+    RB_CUDA(e);
     return ROTOR_B200_OK;
 }
 unsigned* library_status_word() { return ensure_status() ? nullptr : g_status_words.here(); }

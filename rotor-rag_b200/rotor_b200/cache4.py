@@ -37,6 +37,7 @@ class Cache4:
         self.k_step, self.k_least, self.v_step, self.v_least = (make(dim // GROUP, torch.float16) for _ in range(4))
         self._c = abi.Cache4(batch, kv_heads, self.max_seq, dim, *(t.data_ptr() for t in self._tensors()))
         self._ref = C.byref(self._c)
+        self._device = self.k_codes.get_device()
 
     def _tensors(self):
         return self.k_codes, self.v_codes, self.k_step, self.k_least, self.v_step, self.v_least
@@ -50,6 +51,12 @@ class Cache4:
         """``ops.reorder_states`` of this cache: sequence b * width + w becomes what b * width + beams[b, w] was, in its first
         ``length`` positions (all of them unless given)."""
         reorder_states(self.states(), beams, None if length is None else min(-(-length // 16) * 16, self.max_seq))
+
+    def _here(self):
+        device, stream = abi.device_and_stream()
+        if device != self._device:
+            raise ValueError(f"the cache is on {self.k_codes.device}, not on the current CUDA device")
+        return device, stream
 
     def _past(self, past, seq, device):
         """(number, address of the lengths or None), checked."""
@@ -78,7 +85,7 @@ class Cache4:
     def append(self, k, v, past):
         """Rows k and v [batch, seq, kv_heads, dim] (float32, bfloat16 or float16, any strides with columns side by side) are quantised
         into the positions from ``past`` on; with a tensor of lengths, positions behind the end of the cache are left out."""
-        device, stream = abi.device_and_stream()
+        device, stream = self._here()
         ks, vs = self._rows("k", k, self.kv_heads, device), self._rows("v", v, self.kv_heads, device)
         seq = k.shape[1]
         if seq != v.shape[1] or k.dtype is not v.dtype:
@@ -92,7 +99,7 @@ class Cache4:
 
     def read(self, begin: int, end: int, dtype=None):
         """What positions begin .. end - 1 stand for: keys and values [batch, kv_heads, end - begin, dim] (float32 unless told)."""
-        _, stream = abi.device_and_stream()
+        _, stream = self._here()
         dtype = dtype or abi._torch.float32
         if not 0 <= begin <= end <= self.max_seq:
             raise ValueError(f"positions {begin} to {end} of a cache of {self.max_seq}")
@@ -113,7 +120,7 @@ class Cache4:
         query sees that many positions, its own included.  ``sinks`` float32 [heads]: exp(sink) joins the softmax's denominator.
         ``longest``: with a tensor of lengths, the most that a sequence holds, by which the work is divided (the cache's size unless
         given); longer lengths are taken as it.  A query that sees no position gives zeros."""
-        device, stream = abi.device_and_stream()
+        device, stream = self._here()
         heads = q.shape[2] if q.dim() == 4 else 0
         strides = self._rows("q", q, heads, device)
         if heads < 1 or heads % self.kv_heads:

@@ -256,7 +256,7 @@ def reorder_states(states, beams, length=None):
     ``beam_select`` the caches and histories follow the beams they continue.
 
     ``states``: tensors [groups * width, ...] whose rows are contiguous, or pairs (tensor, axis) of which the first ``length`` positions
-    along that axis move.  ``beams`` int64 [groups, width], up to 32 wide; rows whose beam is their own, or none of the group, stay."""
+    along that axis move; their memory may not overlap.  ``beams`` int64 [groups, width], up to 32 wide; rows whose beam is their own, or none of the group, stay."""
     device, stream = abi.device_and_stream()
     on_device("beams", beams, device, 2, abi._torch.int64)
     groups, width = beams.shape

@@ -371,6 +371,81 @@ def test_repeated_calls_give_the_same_bits(torch):
             assert torch.equal(cache.attend(q, 900), first)
 
 
+def test_prompts_a_few_sequences_at_a_time(torch):
+    """Dense rows of more than a GiB are made for some of the sequences at a time: each gets the bits that it gets alone."""
+    from rotor_b200 import abi, ops
+    from rotor_b200.cache4 import Cache4
+    batch, kv, room, dim, heads, seq = 5, 8, 65536 + 256, 128, 32, 256
+    torch.manual_seed(5)
+    cache = Cache4(batch, kv, room, dim)
+    for at in range(0, room, 4096):
+        k, v = (torch.randn((batch, min(4096, room - at), kv, dim), device="cuda", dtype=torch.bfloat16) for _ in range(2))
+        cache.append(k, v, at)
+    q = torch.randn((batch, seq, heads, dim), device="cuda", dtype=torch.bfloat16)
+    past = torch.tensor([65536, 100, 40000, 0, 65000], dtype=torch.int32, device="cuda")
+    each = 4 * kv * (65536 + seq) * dim
+    bytes_of = lambda c: abi.lib.rotor_b200_cache4_attend_workspace_bytes(c._ref, ops.type_code(q.dtype), heads, seq, 65536, 0)
+    assert 3 * each < bytes_of(cache) < 4 * each
+    got = cache.attend(q, past, longest=65536)
+    for b in range(batch):
+        alone = Cache4(1, kv, room, dim)
+        for mine, all_ in zip(alone._tensors(), cache._tensors()):
+            mine.copy_(all_[b:b + 1])
+        assert each <= bytes_of(alone) < 2 * each
+        assert torch.equal(alone.attend(q[b:b + 1], past[b:b + 1], longest=65536), got[b:b + 1]), b
+
+
+def test_another_device_is_refused(torch):
+    from rotor_b200.cache4 import Cache4
+    cache = Cache4(1, 1, 16, 32)
+    x = torch.zeros((1, 1, 1, 32), device="cuda")
+    cache._device += 1
+    for call in (lambda: cache.append(x, x, 0), lambda: cache.read(0, 1), lambda: cache.attend(x, 0)):
+        with pytest.raises(ValueError, match="current CUDA device"):
+            call()
+
+
+FRESH = """
+import torch
+from rotor_b200 import ops
+from rotor_b200.cache4 import Cache4
+torch.manual_seed(3)
+def calls():
+    cache = Cache4(8, 2, 400, 128)
+    k, v = (torch.randn((8, 300, 2, 128), device="cuda", dtype=torch.bfloat16) for _ in range(2))
+    q = torch.randn((8, 300, 8, 128), device="cuda", dtype=torch.bfloat16)
+    wide = torch.randn((16, 8, 40000), device="cuda")
+    one = torch.randn((1, 2, 500), device="cuda")
+    scores = torch.zeros((16, 8), device="cuda")
+    def run():
+        cache.append(k, v, 0)
+        return (*cache.read(0, 300), cache.attend(q, 0), cache.attend(q[:, :1].contiguous(), 299), *ops.beam_select(wide, scores, 9),
+                *ops.beam_select(one, scores[:1, :2], 3))
+    return run
+run = calls()
+torch.cuda.synchronize()
+graph = torch.cuda.CUDAGraph()
+with torch.cuda.graph(graph):
+    got = run()
+graph.replay()
+graph.replay()
+torch.cuda.synchronize()
+assert all(torch.equal(a, b) for a, b in zip(got, run()))
+print("same")
+"""
+
+
+def test_the_first_call_of_a_process_may_be_captured(torch):
+    import os
+    import subprocess
+    import sys
+    import rotor_b200
+    here = os.path.dirname(os.path.dirname(rotor_b200.__file__))
+    r = subprocess.run([sys.executable, "-c", FRESH], capture_output=True, text=True, timeout=300,
+                       env=dict(os.environ, PYTHONPATH=here + os.pathsep + os.environ.get("PYTHONPATH", "")))
+    assert r.returncode == 0 and r.stdout.strip() == "same", r.stderr[-2000:]
+
+
 def test_refusals(torch):
     from rotor_b200.cache4 import Cache4
     cache = Cache4(2, 2, 32, 64)
