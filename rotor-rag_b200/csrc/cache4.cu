@@ -1,12 +1,16 @@
 // The 4-bit cache is written and read back (layout: cache4.cuh).  Both directions move bytes: of a bf16 row of 128 columns 256 bytes
 // on the dense side and 80 in the cache.  A thread takes eight neighbouring columns of four positions (a multiple of four and the next
 // three): those are one word of each key row or two 8-byte words of a value tile, four threads are a group, and threads run along rows.
-// Four rows a thread keep enough loads in flight, and values leave in pieces of 8 bytes instead of 2.
+// Four rows a thread keep enough loads in flight, and values leave in pieces of 8 bytes instead of 2.  Measured, 163840 rows of 128 columns
+// (2 x 8 x 2048 x 5): written from bf16 in 19.0 us (2.9 TB/s; 19 instructions a column and the wait for a thread's one round of loads bound it;
+// with the columns as float32 in registers, 62 of them, 26), from float32 in 18.1 (5.4 TB/s); read as bf16 in 9.9 us (5.6 TB/s).
+#include <type_traits>
+
 #include "cache4.cuh"
 
 namespace rb {
 
-constexpr int C4_THREADS = 256;
+constexpr int C4_THREADS = 128;
 
 // Where eight columns (c8 of a row) of positions quad .. quad + 3 lie.  Keys: a word, `next` bytes to the next position; values: four 16-bit
 // words in a row, and `next` bytes behind them those of the next part g.  group: s and m of the first position, group_next to the next.
@@ -58,19 +62,69 @@ __device__ __forceinline__ float fast_rcp(float x) {
     return y;
 }
 
-// Smallest and largest of the groups of four rows x[k], of which each of four neighbouring threads holds eight columns: thread t of the
-// four gets those of row t.  (Rows are handed over by halves, so that every thread makes one row's s and m and not all four.)
-__device__ __forceinline__ void group_bounds(const float (&x)[4][8], int t, float& low, float& high) {
-    float lo[4], hi[4];
+// Eight neighbouring columns as they came: 16-bit ones stay two in a word until they are needed (half the registers, and a minimum of two is
+// one instruction).
+template <typename T>
+struct Eight {
+    uint32_t w[4];
+    using Two = typename std::conditional<std::is_same<T, __half>::value, __half2, __nv_bfloat162>::type;
+    __device__ __forceinline__ Two two(int n) const { return *reinterpret_cast<const Two*>(&w[n]); }
+    __device__ __forceinline__ void none() { w[0] = w[1] = w[2] = w[3] = 0u; }
+    __device__ __forceinline__ void load(const T* p, bool wide) {
+        if (wide) {
+            const uint4 v = *reinterpret_cast<const uint4*>(p);
+            w[0] = v.x, w[1] = v.y, w[2] = v.z, w[3] = v.w;
+        } else {
+            const uint16_t* h = reinterpret_cast<const uint16_t*>(p);
 #pragma unroll
-    for (int k = 0; k < 4; ++k) {  // (minimum and maximum pass over NaN)
-        lo[k] = hi[k] = x[k][0];
-#pragma unroll
-        for (int n = 1; n < 8; ++n) {
-            lo[k] = fminf(lo[k], x[k][n]);
-            hi[k] = fmaxf(hi[k], x[k][n]);
+            for (int n = 0; n < 4; ++n) w[n] = h[2 * n] | (uint32_t)h[2 * n + 1] << 16;
         }
     }
+    // (minimum and maximum pass over NaN)
+    __device__ __forceinline__ void bounds(float& lo, float& hi) const {
+        const Two a = __hmin2(__hmin2(two(0), two(1)), __hmin2(two(2), two(3))), b = __hmax2(__hmax2(two(0), two(1)), __hmax2(two(2), two(3)));
+        lo = fminf(type_load(&a.x), type_load(&a.y));
+        hi = fmaxf(type_load(&b.x), type_load(&b.y));
+    }
+    __device__ __forceinline__ float2 pair(int n) const {
+        const Two a = two(n);
+        return make_float2(type_load(&a.x), type_load(&a.y));
+    }
+};
+template <>
+struct Eight<float> {
+    float x[8];
+    __device__ __forceinline__ void none() {
+#pragma unroll
+        for (int n = 0; n < 8; ++n) x[n] = 0.f;
+    }
+    __device__ __forceinline__ void load(const float* p, bool wide) {
+        if (wide) {
+            const float4 a = *reinterpret_cast<const float4*>(p), b = *reinterpret_cast<const float4*>(p + 4);
+            x[0] = a.x, x[1] = a.y, x[2] = a.z, x[3] = a.w, x[4] = b.x, x[5] = b.y, x[6] = b.z, x[7] = b.w;
+        } else {
+#pragma unroll
+            for (int n = 0; n < 8; ++n) x[n] = p[n];
+        }
+    }
+    __device__ __forceinline__ void bounds(float& lo, float& hi) const {
+        lo = hi = x[0];
+#pragma unroll
+        for (int n = 1; n < 8; ++n) {
+            lo = fminf(lo, x[n]);
+            hi = fmaxf(hi, x[n]);
+        }
+    }
+    __device__ __forceinline__ float2 pair(int n) const { return make_float2(x[2 * n], x[2 * n + 1]); }
+};
+
+// Smallest and largest of the groups of four rows x[k], of which each of four neighbouring threads holds eight columns: thread t of the
+// four gets those of row t.  (Rows are handed over by halves, so that every thread makes one row's s and m and not all four.)
+template <typename T>
+__device__ __forceinline__ void group_bounds(const Eight<T> (&x)[4], int t, float& low, float& high) {
+    float lo[4], hi[4];
+#pragma unroll
+    for (int k = 0; k < 4; ++k) x[k].bounds(lo[k], hi[k]);
     const bool up = t & 2, odd = t & 1;
     float l[2], h[2];
 #pragma unroll
@@ -91,7 +145,8 @@ __device__ __forceinline__ uint32_t group_params(float low, float high) {
 }
 
 // The codes of eight columns, column n in bits 4 n.
-__device__ __forceinline__ uint32_t quantise8(const float (&x)[8], uint32_t params) {
+template <typename T>
+__device__ __forceinline__ uint32_t quantise8(const Eight<T>& x, uint32_t params) {
     const float2 sm = __half22float2(*reinterpret_cast<const __half2*>(&params));
     const float s = sm.x, m = sm.y, inv = s > 0.f ? fast_rcp(s) : 0.f, inv15 = inv * (1.f / 15.f);
     // the quotient over 15, kept within 0 .. 1 (NaN: 0); 1.5 2^23 + 15 times that is a whole number, to the nearest, ties to even
@@ -102,24 +157,27 @@ __device__ __forceinline__ uint32_t quantise8(const float (&x)[8], uint32_t para
     float off = 0.f;
 #pragma unroll
     for (int n = 0; n < 4; ++n) {
-        const float2 d = __fadd2_rn(make_float2(x[2 * n], x[2 * n + 1]), minus_m);
+        const float2 d = __fadd2_rn(x.pair(n), minus_m);
         const float2 q = make_float2(__saturatef(d.x * inv15), __saturatef(d.y * inv15));
         code[n] = __fadd2_rn(__ffma2_rn(q, fifteen, to_whole), back);
         const float2 e = __ffma2_rn(code[n], minus, __fmul2_rn(q, fifteen));
         off = fmaxf(off, fmaxf(fabsf(e.x), fabsf(e.y)));
     }
-    // The quotient in float32 is off by less than 1e-5: what lies that near to a border k + 1/2 between two codes is compared with it in
-    // 64 bits, where x - m and (k + 1/2) s have room.  (Types of few bits come here often: (x - m) / s is a ratio of small numbers, and of
-    // 256 bf16 columns one lies on a border in a seventh of the cases.)
+    // The quotient in float32 is off by less than 1e-5: of what lies that near to a border k + 1/2 between two codes, x - m is compared with
+    // (k + 1/2) s exactly: that is a product of 11 and 5 bits, x - m is the sum of its rounded value and of what the rounding left, and the
+    // difference of two numbers that near to one another is exact.  (Types of few bits come here often: (x - m) / s is a ratio of small
+    // numbers, and of 256 bf16 columns one lies on a border in a seventh of the cases.)
     if (off > 0.5f - 2e-5f) {
 #pragma unroll
         for (int n = 0; n < 8; ++n) {
             float& c = n & 1 ? code[n >> 1].y : code[n >> 1].x;
-            const float q = fminf(fmaxf((x[n] - m) * inv, 0.f), 15.f);
+            const float2 two = x.pair(n >> 1);
+            const float value = n & 1 ? two.y : two.x, q = fminf(fmaxf((value - m) * inv, 0.f), 15.f);
             if (fabsf(q - c) > 0.5f - 4e-5f) {
                 const float below = floorf(q);
-                const double d = fma(-((double)below + 0.5), (double)s, (double)x[n] - (double)m);
-                c = below + (d > 0.0 || (d == 0.0 && ((int)below & 1)) ? 1.f : 0.f);
+                const float t = value - m, taken = t - value, left = (value - (t - taken)) - (m + taken);
+                const float d = (t - (below + 0.5f) * s) + left;
+                c = below + (d > 0.f || (d == 0.f && ((int)below & 1)) ? 1.f : 0.f);
             }
         }
     }
@@ -134,7 +192,7 @@ __device__ __forceinline__ uint32_t quantise8(const float (&x)[8], uint32_t para
 }
 
 template <typename T>
-__global__ void __launch_bounds__(C4_THREADS, 4) cache4_store_kernel(const __grid_constant__ Cache4Store p) {
+__global__ void __launch_bounds__(C4_THREADS, sizeof(T) == 4 ? 8 : 10) cache4_store_kernel(const __grid_constant__ Cache4Store p) {
     pdl_wait();
     pdl_trigger();
     const uint32_t u = blockIdx.x * C4_THREADS + threadIdx.x;
@@ -145,15 +203,11 @@ __global__ void __launch_bounds__(C4_THREADS, 4) cache4_store_kernel(const __gri
     const int past = past_of(p.past, b), quad = (past & ~3) + 4 * (int)nth;
     const int from = max(past - quad, 0), to = min(min(past + p.seq, p.c.max_seq) - quad, 4);  // which of the four are there
     const T* src = static_cast<const T*>(p.src[part]) + (size_t)b * p.sb[part] + (size_t)h * p.sh[part] + c8 * 8;
-    float x[4][8];
+    Eight<T> x[4];
 #pragma unroll
     for (int k = 0; k < 4; ++k) {
-        if (k >= from && k < to) {
-            load8(src + (size_t)(quad + k - past) * p.ss[part], p.wide[part], x[k]);
-        } else {
-#pragma unroll
-            for (int n = 0; n < 8; ++n) x[k][n] = 0.f;
-        }
+        if (k >= from && k < to) x[k].load(src + (size_t)(quad + k - past) * p.ss[part], p.wide[part]);
+        else x[k].none();
     }
     float low, high;
     group_bounds(x, c8 & 3, low, high);
