@@ -180,7 +180,7 @@ class State(C.Structure):
     _fields_ = [("data", _p), ("row_stride", _sz), ("segment_stride", _sz), ("segment_bytes", _sz), ("segments", C.c_int32)]
 
 
-_c4p, _i64, _sdp = C.POINTER(Cache4), C.c_int64, C.POINTER(C.c_int64)
+_c4p, _i64, _sdp = C.POINTER(Cache4), C.c_int64, C.c_void_p   # (_sdp: a host array of strides, or its bytes)
 
 _SIGNATURES.update({
     "rotor_b200_beam_select_workspace_bytes": (_sz, [_i, _i, _i, _i, _i]),

@@ -7,13 +7,14 @@ reads the codes themselves.
 from __future__ import annotations
 
 import ctypes as C
+import struct
 
 from . import abi
 from .abi import check, lib
 from .ops import on_device, reorder_states, type_code
 
 GROUP = 32
-_Strides = C.c_int64 * 3
+_strides = struct.Struct("3q").pack     # (of sequence, position and head, as the C entry points take them)
 DIMS = (32, 64, 96, 128, 192, 256)
 
 
@@ -72,23 +73,24 @@ class Cache4:
         return past, None
 
     def _rows(self, name, x, heads, device):
-        """Strides of rows [batch, seq, heads, dim], checked."""
-        on_device(name, x, device, 4)
-        b, s, h, d = x.shape
+        """Positions and strides of rows [batch, seq, heads, dim], checked."""
+        shape = x.shape
+        if x.get_device() != device or len(shape) != 4:
+            on_device(name, x, device, 4)
+        b, s, h, d = shape
         if b != self.batch or h != heads or d != self.dim:
             raise ValueError(f"{name} of shape {(b, s, h, d)}, expected {(self.batch, 'positions', heads, self.dim)}")
         sb, ss, sh, sd = x.stride()
         if sd != 1:
             raise ValueError(f"the columns of {name} have to lie side by side")
-        return _Strides(sb, ss, sh)
+        return s, _strides(sb, ss, sh)
 
     def append(self, k, v, past):
         """Rows k and v [batch, seq, kv_heads, dim] (float32, bfloat16 or float16, any strides with columns side by side) are quantised
         into the positions from ``past`` on; with a tensor of lengths, positions behind the end of the cache are left out."""
         device, stream = self._here()
-        ks, vs = self._rows("k", k, self.kv_heads, device), self._rows("v", v, self.kv_heads, device)
-        seq = k.shape[1]
-        if seq != v.shape[1] or k.dtype is not v.dtype:
+        (seq, ks), (v_seq, vs) = self._rows("k", k, self.kv_heads, device), self._rows("v", v, self.kv_heads, device)
+        if seq != v_seq or k.dtype is not v.dtype:
             raise ValueError(f"k is {k.dtype} {tuple(k.shape)}, v is {v.dtype} {tuple(v.shape)}")
         code = type_code(k.dtype)
         number, lengths = self._past(past, seq, device)
@@ -122,10 +124,10 @@ class Cache4:
         given); longer lengths are taken as it.  A query that sees no position gives zeros."""
         device, stream = self._here()
         heads = q.shape[2] if q.dim() == 4 else 0
-        strides = self._rows("q", q, heads, device)
+        seq, strides = self._rows("q", q, heads, device)
         if heads < 1 or heads % self.kv_heads:
             raise ValueError(f"{heads} query heads cannot share {self.kv_heads} key/value heads evenly")
-        code, seq = type_code(q.dtype), q.shape[1]
+        code = type_code(q.dtype)
         number, lengths = self._past(past, seq, device)
         if window < 0:
             raise ValueError(f"a window of {window} positions")
@@ -139,15 +141,12 @@ class Cache4:
             return out
         bound = number if lengths is None else self.max_seq if longest is None else min(max(int(longest), 0), self.max_seq)
         scale = self.dim ** -0.5 if scale is None else float(scale)
-
-        def call(workspace, size):
-            return lib.rotor_b200_cache4_attend(self._ref, q.data_ptr(), code, strides, heads, seq, number, lengths, bound, scale, window, sinks,
-                                                out.data_ptr(), workspace, size, stream)
-        status = call(None, 0)
+        call = self._ref, q.data_ptr(), code, strides, heads, seq, number, lengths, bound, scale, window, sinks, out.data_ptr()
+        status = lib.rotor_b200_cache4_attend(*call, None, 0, stream)
         if status == abi.ERR_WORKSPACE:      # (nothing has been launched; few tokens need none)
             need = lib.rotor_b200_cache4_attend_workspace_bytes(self._ref, code, heads, seq, bound, window)
             workspace = q.new_empty(need, dtype=abi._torch.uint8)
-            status = call(workspace.data_ptr(), need)
+            status = lib.rotor_b200_cache4_attend(*call, workspace.data_ptr(), need, stream)
         if status:
             check(status, "cache4_attend")
         return out

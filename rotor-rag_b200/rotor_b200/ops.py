@@ -225,7 +225,8 @@ def beam_select(logits, scores, count, ended=None, pad=0):
         if not 0 <= pad < vocab:
             raise ValueError(f"padding token {pad} of {vocab}")
         ended = ended.contiguous()
-    scores = scores.contiguous()
+    if not scores.is_contiguous():
+        scores = scores.contiguous()
     shape = (groups, count)
     best = scores.new_empty(shape)
     beams = scores.new_empty(shape, dtype=torch.int64)
@@ -234,15 +235,13 @@ def beam_select(logits, scores, count, ended=None, pad=0):
         return best, beams, tokens
     if groups * width > 65535:
         raise ValueError(f"{groups} groups of {width} beams: up to 65535 beams in a call")
-    def call(workspace, size):
-        return lib.rotor_b200_beam_select(logits.data_ptr(), code, group_stride, beam_stride, scores.data_ptr(),
-                                          None if ended is None else ended.data_ptr(), groups, width, vocab, count, int(pad),
-                                          best.data_ptr(), beams.data_ptr(), tokens.data_ptr(), workspace, size, stream)
-    status = call(None, 0)
+    call = (logits.data_ptr(), code, group_stride, beam_stride, scores.data_ptr(), None if ended is None else ended.data_ptr(), groups, width,
+            vocab, count, int(pad), best.data_ptr(), beams.data_ptr(), tokens.data_ptr())
+    status = lib.rotor_b200_beam_select(*call, None, 0, stream)
     if status == abi.ERR_WORKSPACE:      # (nothing has been launched; few logits need none)
         need = lib.rotor_b200_beam_select_workspace_bytes(code, groups, width, vocab, count)
         workspace = scores.new_empty(need, dtype=torch.uint8)
-        status = call(workspace.data_ptr(), need)
+        status = lib.rotor_b200_beam_select(*call, workspace.data_ptr(), need, stream)
     if status:
         check(status, "beam_select")
     return best, beams, tokens
