@@ -19,7 +19,8 @@
 // a barrier operation queues behind the special function unit's, 250 clocks).  Measured, bf16, 32 query and 8 KV heads of 128, causal, with the
 // dense rows made first: 8192 tokens of one sequence 508 us (1.08 PFLOP/s), 8 x 2048 tokens of 20 and 5 heads 190 us (0.91), float16 216.
 // Tried and slower: weights in one piece (3%); half or a quarter of the exponentials by polynomials in the FMA pipe (10%, 0%); steps of 64
-// keys with two score blocks in flight for each block (30%: twice the barriers); items in the same order for every round of CTAs (8%).
+// keys with two score blocks in flight for each block (30%: twice the barriers); items in the same order for every round of CTAs (8%); weights
+// against the last reference with a look at their sum afterwards, without the tile's maximum (4 to 9%).
 // Rounded to the 16-bit type, beside the outputs: keys and values as dense rows (the tensor cores' operands) and weights (at most 2^8, their
 // sum is of unrounded ones); scores, maxima, sums and outputs are float32.
 // Waits are bounded; a wait that runs out records a code in the library status word, the CTA stops issuing work, frees its tensor memory
