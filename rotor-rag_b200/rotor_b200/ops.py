@@ -265,12 +265,14 @@ def reorder_states(states, beams, length=None):
     described, addresses = [], set()
     for s in states:
         t, axis = s if isinstance(s, tuple) else (s, None)
-        shape, size = t.shape, t.element_size()
+        if length is None:
+            axis = None
+        shape = t.shape
         if t.get_device() != device:
             raise ValueError(f"a state is on {t.device}, not on the current CUDA device")
         if not shape or shape[0] != rows:
             raise ValueError(f"a state of shape {tuple(shape)} for {groups} x {width} beams")
-        if axis is not None and length is not None:
+        if axis is not None:
             if not 1 <= axis < len(shape):
                 raise ValueError(f"positions along axis {axis} of a state of {len(shape)} dimensions")
             if not 0 <= length <= shape[axis]:
@@ -278,23 +280,24 @@ def reorder_states(states, beams, length=None):
         n = t.numel()
         if n == 0:
             continue
-        row = piece = part = n // rows * size
-        row_stride = row
+        size = t.element_size()
+        row = row_stride = n // rows * size
         if not t.is_contiguous():
             row_stride = t.stride(0) * size
             if not t[0].is_contiguous() or (rows > 1 and row_stride < row):
                 raise ValueError(f"a state's rows have to be contiguous and apart; got shape {tuple(shape)}, strides {t.stride()}")
-        if axis is not None and length is not None:
-            inner = size
-            for k in shape[axis + 1:]:
-                inner *= k
-            piece, part = shape[axis] * inner, length * inner
         address = t.data_ptr()
         if address in addresses:
             raise ValueError("the same state twice")
         addresses.add(address)
-        if part:
-            described.append(_STATE.pack(address, row_stride, piece, part, row // piece))
+        if axis is None:
+            described.append(_STATE.pack(address, row_stride, row, row, 1))
+        elif length:
+            segments = 1          # (pieces of a row: what lies in front of the axis)
+            for k in range(1, axis):
+                segments *= shape[k]
+            piece = row // segments
+            described.append(_STATE.pack(address, row_stride, piece, piece // shape[axis] * length, segments))
     if not described:
         return
     beams = beams.contiguous()
