@@ -399,6 +399,28 @@ def test_prompts_a_few_sequences_at_a_time(torch):
         assert torch.equal(alone.attend(q[b:b + 1], past[b:b + 1], longest=65536), got[b:b + 1]), b
 
 
+def test_offsets_beyond_32_bits(torch):
+    """The last sequence's codes lie 5.3 GB behind the first one's, and the same rows give the same bits there."""
+    from rotor_b200.cache4 import Cache4
+    torch.manual_seed(6)
+    batch, room = 80, 131072
+    cache = Cache4(batch, 8, room, 128)
+    assert (batch - 1) * cache.k_codes.stride(0) > 2 ** 32
+    k, v = (torch.randn((1, 600, 8, 128), device="cuda", dtype=torch.bfloat16).expand(batch, -1, -1, -1) for _ in range(2))
+    cache.append(k, v, room - 600)
+    for rows, held in zip(cache.read(room - 600, room, dtype=torch.float32), (k, v)):
+        assert torch.equal(rows[0], rows[-1]) and (rows[0] - held[0].transpose(0, 1)).abs().max() < 1.0
+    for seq in (1, 9, 200):
+        q = torch.randn((1, seq, 64, 128), device="cuda", dtype=torch.bfloat16).expand(batch, -1, -1, -1)
+        for x in (q, q.contiguous()):
+            out = cache.attend(x, room - seq, window=700)
+            assert torch.equal(out[0], out[-1]) and out[0].abs().max() > 0
+    mark = cache.v_codes[-1, :, -16:].clone()
+    cache.v_codes[-8, :, -16:] = 0
+    cache.reorder(torch.arange(8, device="cuda").flip(0).repeat(batch // 8, 1))
+    assert torch.equal(cache.v_codes[-8, :, -16:], mark) and not cache.v_codes[-1, :, -16:].any()
+
+
 def test_another_device_is_refused(torch):
     from rotor_b200.cache4 import Cache4
     cache = Cache4(1, 1, 16, 32)
