@@ -421,6 +421,23 @@ def test_offsets_beyond_32_bits(torch):
     assert torch.equal(cache.v_codes[-8, :, -16:], mark) and not cache.v_codes[-1, :, -16:].any()
 
 
+@pytest.mark.parametrize("dtype", TYPES)
+def test_reading_to_any_address(torch, dtype):
+    """Buffers that begin at multiples of 16 bytes, and not of 32, get the same bits."""
+    from rotor_b200 import abi, ops
+    from rotor_b200.cache4 import Cache4
+    cache = Cache4(2, 3, 50, 96)
+    cache.append(*make(torch, np.random.default_rng(9), (2, 2, 40, 3, 96), dtype), 5)
+    want = cache.read(3, 41, dtype=getattr(torch, dtype))
+    off = 16 // want[0].element_size()
+    got = [torch.full((want[0].numel() + 2 * off,), 7.0, dtype=want[0].dtype, device="cuda") for _ in range(2)]
+    assert all(g.data_ptr() % 32 == 0 for g in got)
+    status = abi.lib.rotor_b200_cache4_read(cache._ref, 3, 41, got[0][off:].data_ptr(), got[1].data_ptr(), ops.type_code(want[0].dtype), abi.stream())
+    assert status == 0
+    for g, w, at in zip(got, want, (off, 0)):
+        assert torch.equal(g[at:at + w.numel()], w.reshape(-1)) and (g[:at] == 7).all() and (g[at + w.numel():] == 7).all()
+
+
 def test_another_device_is_refused(torch):
     from rotor_b200.cache4 import Cache4
     cache = Cache4(1, 1, 16, 32)
