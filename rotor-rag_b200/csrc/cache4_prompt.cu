@@ -18,9 +18,10 @@
 // 550 instructions a warp, and the other block's warps share the schedulers) -> sums -> next scores (1024 clocks of MMA, some 600 of barriers:
 // a barrier operation queues behind the special function unit's, 250 clocks).  Measured, bf16, 32 query and 8 KV heads of 128, causal, with the
 // dense rows made first: 8192 tokens of one sequence 508 us (1.08 PFLOP/s), 8 x 2048 tokens of 20 and 5 heads 190 us (0.91), float16 216.
-// Tried and slower: weights in one piece (3%); half or a quarter of the exponentials by polynomials in the FMA pipe (10%, 0%); steps of 64
-// keys with two score blocks in flight for each block (30%: twice the barriers); items in the same order for every round of CTAs (8%); weights
-// against the last reference with a look at their sum afterwards, without the tile's maximum (4 to 9%).
+// Tried and slower: outputs by 16 bytes (3%: halves of sectors); weights in one piece (3%); half or a quarter of the exponentials by
+// polynomials in the FMA pipe (10%, 0%); steps of 64 keys with two score blocks in flight for each block (30%: twice the barriers); items in
+// the same order for every round of CTAs (8%); weights against the last reference with a look at their sum afterwards, without the tile's
+// maximum (4 to 9%).
 // Rounded to the 16-bit type, beside the outputs: keys and values as dense rows (the tensor cores' operands) and weights (at most 2^8, their
 // sum is of unrounded ones); scores, maxima, sums and outputs are float32.
 // Waits are bounded; a wait that runs out records a code in the library status word, the CTA stops issuing work, frees its tensor memory
@@ -49,6 +50,7 @@ struct P4Params {
     unsigned* status;
     int heads, kv_heads, dim, seq, span, max_seq, window;
     int blocks, items;              // of 2 x 128 rows: of a sequence's KV head, of the call
+    bool whole;                     // outputs begin at a multiple of 32 bytes
     float scale2;                   // |scale| log2(e) (its sign is in the keys)
 };
 
@@ -229,11 +231,18 @@ cache4_prompt_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_cons
                 }
                 if (real && c < p.dim) {
 #pragma unroll
-                    for (int i = 0; i < 32; i += 8) {
-                        uint32_t v[4];
+                    for (int i = 0; i < 32; i += 16) {
+                        uint32_t v[8];
 #pragma unroll
-                        for (int n = 0; n < 4; ++n) v[n] = p4_pack<HALF>(__uint_as_float(o[i + 2 * n]) * inv, __uint_as_float(o[i + 2 * n + 1]) * inv);
-                        *reinterpret_cast<uint4*>(out + c + i) = make_uint4(v[0], v[1], v[2], v[3]);
+                        for (int n = 0; n < 8; ++n) v[n] = p4_pack<HALF>(__uint_as_float(o[i + 2 * n]) * inv, __uint_as_float(o[i + 2 * n + 1]) * inv);
+                        if (p.whole) {
+                            asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(out + c + i), "r"(v[0]), "r"(v[1]), "r"(v[2]),
+                                         "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7])
+                                         : "memory");
+                        } else {
+                            *reinterpret_cast<uint4*>(out + c + i) = make_uint4(v[0], v[1], v[2], v[3]);
+                            *reinterpret_cast<uint4*>(out + c + i + 8) = make_uint4(v[4], v[5], v[6], v[7]);
+                        }
                     }
                 }
             }
@@ -407,6 +416,7 @@ int launch_prompt_attn(const PromptAttn& p, cudaStream_t st) {
     if (!prompt_attn_supported(p.batch, p.heads, p.kv_heads, p.dim, p.span)) return ROTOR_B200_ERR_SHAPE;
     P4Params a = {};
     a.out = static_cast<uint16_t*>(p.out);
+    a.whole = ((uintptr_t)p.out & 31) == 0;
     a.past_len = p.past_len;
     a.sinks = p.sinks;
     a.status = library_status_word();

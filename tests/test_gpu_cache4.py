@@ -438,6 +438,25 @@ def test_reading_to_any_address(torch, dtype):
         assert torch.equal(g[at:at + w.numel()], w.reshape(-1)) and (g[:at] == 7).all() and (g[at + w.numel():] == 7).all()
 
 
+def test_prompts_to_any_address(torch):
+    """Outputs that begin at a multiple of 16 bytes, and not of 32, get the same bits, and nothing beside them is written."""
+    import ctypes as C
+    from rotor_b200 import abi, ops
+    from rotor_b200.cache4 import Cache4
+    torch.manual_seed(8)
+    cache = Cache4(8, 2, 300, 64)
+    cache.append(*torch.randn((2, 8, 300, 2, 64), device="cuda"), 0)
+    q = torch.randn((8, 300, 16, 64), device="cuda", dtype=torch.bfloat16)
+    want, code, n = cache.attend(q, 0), ops.type_code(q.dtype), q.numel()
+    need = abi.lib.rotor_b200_cache4_attend_workspace_bytes(cache._ref, code, 16, 300, 0, 0)
+    assert need >= 4 * 8 * 2 * 300 * 64
+    work, out = torch.empty(need, dtype=torch.uint8, device="cuda"), torch.full((n + 16,), 7.0, dtype=q.dtype, device="cuda")
+    status = abi.lib.rotor_b200_cache4_attend(cache._ref, q.data_ptr(), code, (C.c_int64 * 3)(*q.stride()[:3]), 16, 300, 0, None, 0, 64 ** -0.5, 0,
+                                              None, out[8:].data_ptr(), work.data_ptr(), need, abi.stream())
+    assert status == 0 and out.data_ptr() % 32 == 0
+    assert torch.equal(out[8:n + 8].view_as(want), want) and (out[:8] == 7).all() and (out[n + 8:] == 7).all()
+
+
 def test_another_device_is_refused(torch):
     from rotor_b200.cache4 import Cache4
     cache = Cache4(1, 1, 16, 32)
