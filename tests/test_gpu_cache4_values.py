@@ -1,0 +1,119 @@
+"""GPU: the 4-bit cache and its attention where values are very small, very large or outweighed, and prompts against a bound that holds
+the roundings the prompt kernel states.
+
+Prompts on dense rows: keys and values are given to the oracle as the kernel has them, rounded through float32 to the type (float16: at most
+65504), so that what is left is
+ * a score: products accumulated in float32 over at most 128 columns, 2^-17 of the sum of |q| |k| (and of one), twice with the ratio to the sum;
+ * the weights' rounding to the type, h = finfo(type).eps / 2 of the weighted sum of |v|; float16 weights below 2^-14 are off by 2^-25:
+   2^-25 of the sum of |v| over the positions;
+ * sums of n positions in float32, 16 at a time: n / 16 additions of 2^-22 at most of the weighted sum of |v|;
+ * the output's rounding, h of it, and of the smallest normal number below that.
+Attention over the codes, 16-bit types: weights and their products with s are float16, 2^-11 with the ratio to the sum, of the weighted sums of
+|v| and of s code, instead of h; the rest as above (scores: the same bound covers eight groups)."""
+import numpy as np
+import pytest
+
+from oracle import cache4_np as O
+
+pytestmark = pytest.mark.gpu
+HALVES = ["bfloat16", "float16"]
+
+
+@pytest.fixture(scope="module")
+def torch():
+    import torch
+    return torch
+
+
+def host(t):
+    return t.float().cpu().numpy().astype(np.float64)
+
+
+def held(x):
+    """Rows [batch, seq, heads, dim] as the cache holds them: [batch, heads, seq, dim]."""
+    return O.held(host(x)).transpose(0, 2, 1, 3)
+
+
+def dense(torch, x, dtype):
+    y = torch.from_numpy(np.clip(x, -65504, 65504) if dtype == "float16" else x).to(torch.float32)
+    return y.to(getattr(torch, dtype)).double().numpy()
+
+
+def rows(torch, rng, shape, dtype, size=1.0):
+    x = (rng.standard_normal(shape) + rng.standard_normal(shape[-2:])) * size
+    return torch.from_numpy(x.astype(np.float32)).cuda().to(getattr(torch, dtype))
+
+
+def needs(torch, cache, dtype, heads, seq, high, window=0):
+    from rotor_b200 import abi, ops
+    return abi.lib.rotor_b200_cache4_attend_workspace_bytes(cache._ref, ops.type_code(getattr(torch, dtype)), heads, seq, high, window)
+
+
+def bound_of(torch, dtype, want, size, reach, weight, many, sum_v, spare):
+    half, tiny = torch.finfo(getattr(torch, dtype)).eps / 2, torch.finfo(getattr(torch, dtype)).smallest_normal
+    return (size * (weight + np.expm1(2.0 ** -16 * (reach[..., None] + 1)) + many / 16 * 2.0 ** -22) + spare * sum_v + half * np.abs(want) + half * tiny
+            + 1e-30)
+
+
+def prompt(torch, seed, dtype, batch, seq, heads, kv, dim, past, window=0, sinks=False, scale=None):
+    """(output, its oracle, the bound); the call is one that goes over dense rows."""
+    from rotor_b200.cache4 import Cache4
+    rng = np.random.default_rng(seed)
+    total = max(past) + seq
+    cache = Cache4(batch, kv, total, dim)
+    assert needs(torch, cache, dtype, heads, seq, max(past), window) >= 4 * batch * kv * total * dim
+    k, v = rows(torch, rng, (batch, total, kv, dim), "bfloat16"), rows(torch, rng, (batch, total, kv, dim), "bfloat16")
+    cache.append(k, v, 0)
+    q = torch.from_numpy(rng.standard_normal((batch, seq, heads, dim)).astype(np.float32)).cuda().to(getattr(torch, dtype))
+    s = torch.from_numpy(rng.standard_normal(heads).astype(np.float32)).cuda() if sinks else None
+    lengths = torch.tensor(past, dtype=torch.int32, device="cuda")
+    got = cache.attend(q, lengths, scale=scale, window=window, sinks=s, longest=max(past))
+    kd, vd = dense(torch, held(k), dtype), dense(torch, held(v), dtype)
+    use = dim ** -0.5 if scale is None else scale
+    args = past, use, window, None if s is None else host(s)
+    want, size, reach = O.attend(host(q), kd, vd, *args)
+    bound = bound_of(torch, dtype, want, size, reach, torch.finfo(getattr(torch, dtype)).eps / 2, total, np.abs(vd).sum(2).max(), 2.0 ** -25)
+    return got, want, bound, (host(q), kd, vd, args)
+
+
+@pytest.mark.parametrize("dtype", HALVES)
+@pytest.mark.parametrize("seq,heads,kv,dim,past,kw", [
+    (300, 20, 5, 128, 0, {}), (300, 6, 6, 96, 77, {}), (300, 8, 2, 32, 3, {}), (260, 8, 2, 128, 300, {"scale": 1.5}), (300, 8, 2, 128, 0, {"scale": 6.0}),
+    (300, 12, 4, 64, 150, {"scale": -9.0, "sinks": True}), (400, 6, 2, 96, 0, {"scale": 3.0}), (300, 8, 1, 128, 300, {"window": 99, "scale": 0.7})])
+def test_prompts_within_the_roundings_that_are_stated(torch, seq, heads, kv, dim, past, kw, dtype):
+    """... and a bound that says something: outputs of zeros, of the next query row, of the next head and without a row's last position
+    are outside of it."""
+    batch = 8
+    got, want, bound, (q, kd, vd, args) = prompt(torch, seq + heads + dim, dtype, batch, seq, heads, kv, dim, [past] * batch, **kw)
+    err = np.abs(host(got) - want)
+    assert np.all(err <= bound), float((err / bound).max())
+    outside = lambda other: (np.abs(other - want) > bound).mean()
+    assert outside(np.zeros_like(want)) > 0.9 and outside(-want) > 0.9
+    assert outside(np.roll(want, 1, 1)) > 0.5 and outside(np.roll(want, 1, 2)) > 0.5
+    if past:      # every row sees a position less: with sharp scores that is the one that counts in one row of so many
+        short = O.attend(q[:1], kd[:1], vd[:1], [past - 1], *args[1:])[0]
+        assert (np.abs(short - want[:1]) > bound[:1]).mean() > 0.5 / (past + seq)
+
+
+@pytest.mark.parametrize("dtype", HALVES)
+@pytest.mark.parametrize("seq,heads,kv,dim,past,kw", [
+    (24, 8, 8, 128, 333, {}), (9, 16, 4, 64, 100, {"scale": 1.0}), (40, 4, 2, 128, 50, {"scale": 3.0}), (20, 12, 3, 96, 80, {"sinks": True, "window": 31}),
+    (30, 4, 2, 256, 60, {"scale": 1.0})])
+def test_portions_over_the_codes(torch, seq, heads, kv, dim, past, kw, dtype):
+    """More than sixteen query rows a KV head, on the kernel that rounds no keys."""
+    from rotor_b200.cache4 import Cache4
+    rng = np.random.default_rng(seq + dim)
+    batch, total, kw = 1, past + seq, dict(kw)
+    cache = Cache4(batch, kv, total, dim)
+    assert needs(torch, cache, dtype, heads, seq, past, kw.get("window", 0)) < 4 * batch * kv * total * dim
+    k, v = rows(torch, rng, (batch, total, kv, dim), "float32"), rows(torch, rng, (batch, total, kv, dim), "float32")
+    cache.append(k, v, 0)
+    q = torch.from_numpy(rng.standard_normal((batch, seq, heads, dim)).astype(np.float32)).cuda().to(getattr(torch, dtype))
+    s = torch.from_numpy(rng.standard_normal(heads).astype(np.float32)).cuda() if kw.pop("sinks", False) else None
+    got = cache.attend(q, past, sinks=s, **kw)
+    want, size, reach = O.attend(host(q), held(k), held(v), [past], kw.get("scale", dim ** -0.5), kw.get("window", 0), None if s is None else host(s),
+                                 O.coded(host(v)).transpose(0, 2, 1, 3))
+    bound = bound_of(torch, dtype, want, size, reach, 2.0 ** -11, total, 0.0, 0.0)
+    err = np.abs(host(got) - want)
+    assert np.all(err <= bound), float((err / bound).max())
+    assert (np.abs(want) > bound).mean() > 0.9
