@@ -137,17 +137,30 @@ __device__ __forceinline__ void group_bounds(const Eight<T> (&x)[4], int t, floa
     high = fmaxf(odd ? h[1] : h[0], __shfl_xor_sync(0xffffffffu, odd ? h[0] : h[1], 1));
 }
 
-// s (low half) and m of a group.  A group of nothing but NaN holds zeros; columns beyond the largest float16 get the outermost codes.
+// s (low half) and m of a group.  A group of nothing but NaN holds zeros.  s is never negative: its sign marks a float32 group with columns
+// above 65504, which are quantised as that.
+constexpr uint32_t C4_BEYOND = 0x8000u;
+template <typename T>
 __device__ __forceinline__ uint32_t group_params(float low, float high) {
     if (low != low) low = high = 0.f;
+    const uint32_t beyond = sizeof(T) == 4 && high > C4_MOST ? C4_BEYOND : 0u;
     low = fminf(fmaxf(low, -C4_MOST), C4_MOST);
     high = fminf(fmaxf(high, -C4_MOST), C4_MOST);
-    return (uint32_t)__half_as_ushort(group_step(low, high)) | (uint32_t)__half_as_ushort(__float2half_rn(low)) << 16;
+    return (uint32_t)__half_as_ushort(group_step(low, high)) | beyond | (uint32_t)__half_as_ushort(__float2half_rn(low)) << 16;
 }
 
 // The codes of eight columns, column n in bits 4 n.
 template <typename T>
-__device__ __forceinline__ uint32_t quantise8(const Eight<T>& x, uint32_t params) {
+__device__ __forceinline__ uint32_t quantise8(Eight<T> x, uint32_t params) {
+    if constexpr (sizeof(T) == 4) {
+        // Where m is rounded up to 65504 or near it, 65504 is not the highest code, which larger columns would get.  (m of 16-bit types
+        // is not rounded and s by 2^-11 at most: 65504 is within a hundredth of the highest code.)
+        if (params & C4_BEYOND) {
+#pragma unroll
+            for (int n = 0; n < 8; ++n) x.x[n] = x.x[n] > C4_MOST ? C4_MOST : x.x[n];  // (NaN stays)
+            params &= ~C4_BEYOND;
+        }
+    }
     const float2 sm = __half22float2(*reinterpret_cast<const __half2*>(&params));
     const float s = sm.x, m = sm.y, inv = s > 0.f ? fast_rcp(s) : 0.f, inv15 = inv * (1.f / 15.f);
     // the quotient over 15, kept within 0 .. 1 (NaN: 0); 1.5 2^23 + 15 times that is a whole number, to the nearest, ties to even
@@ -212,14 +225,14 @@ __global__ void __launch_bounds__(C4_THREADS, sizeof(T) == 4 ? 8 : 10) cache4_st
     }
     float low, high;
     group_bounds(x, c8 & 3, low, high);
-    const uint32_t own = group_params(low, high);
+    const uint32_t own = group_params<T>(low, high);
     uint32_t word[4];
     __half s[4], m[4];
 #pragma unroll
     for (int k = 0; k < 4; ++k) {
         const uint32_t params = __shfl_sync(0xffffffffu, own, (threadIdx.x & 28) + k);
         word[k] = quantise8(x[k], params);
-        s[k] = __ushort_as_half((unsigned short)params);
+        s[k] = __ushort_as_half((unsigned short)(params & ~C4_BEYOND));
         m[k] = __ushort_as_half((unsigned short)(params >> 16));
     }
     if (!on || from >= to) return;

@@ -117,3 +117,25 @@ def test_portions_over_the_codes(torch, seq, heads, kv, dim, past, kw, dtype):
     err = np.abs(host(got) - want)
     assert np.all(err <= bound), float((err / bound).max())
     assert (np.abs(want) > bound).mean() > 0.9
+
+
+def test_magnitudes_above_the_largest_float16(torch):
+    """They are stored as 65504 is: where a group's smallest value rounds up, that is not the highest code."""
+    from rotor_b200.cache4 import Cache4
+    rng = np.random.default_rng(23)
+    x = np.empty((16, 64), np.float32)
+    x[:8] = 65490.0
+    x[8:] = rng.uniform(60000, 65504, (8, 64))
+    x[8:12, :32] = rng.uniform(65400, 65504, (4, 32))
+    big = [70000.0, np.inf, 1e30, 65505.0]
+    for r in range(16):
+        x[r, 5 + r], x[r, 40] = big[r % 4], big[(r + 1) % 4]
+    x[3, 9], x[5, 41] = np.nan, -np.inf
+    for sign in (1, -1):
+        for dtype in ("float32", "bfloat16", "float16"):
+            t = torch.from_numpy((sign * x).reshape(1, 16, 1, 64)).cuda().to(getattr(torch, dtype))
+            cache = Cache4(1, 1, 16, 64)
+            cache.append(t, t.flip(1), 0)
+            k, v = cache.read(0, 16)
+            want = held(t).astype(np.float32).astype(np.float64)
+            assert np.array_equal(host(k), want) and np.array_equal(host(v), want[:, :, ::-1])
