@@ -457,7 +457,8 @@ int rotor_b200_reorder_states(const rotor_b200_state* states, int n, const int64
  * sequence holds already, or, with past_len (device int32 [batch], kept within 0 .. max_seq), past_len[b] of sequence b.
  *  append: k, v `dtype` [batch][seq][kv_heads][dim] go to positions past .. past + seq - 1; those at max_seq and beyond are
  *    not stored.
- *  read: positions begin .. end - 1 of all sequences as k, v `dtype` [batch][kv_heads][end - begin][dim].
+ *  read: positions begin .. end - 1 of all sequences as k, v `dtype` [batch][kv_heads][end - begin][dim].  (m and s are rounded, so
+ *    that m + 15 s can lie above 65504: float16 rows hold 65504 there, and float16 outputs of attend end there, so that finite rows stay finite.)
  *  attend: q `dtype` [batch][seq][heads][dim] sits at positions past .. past + seq - 1 and sees cached positions j <= its own,
  *    with window > 0 those with (own - j) < window.  Softmax of scale * q . k, whose denominator holds exp(sinks[head]) as well
  *    (sinks float32 [heads] or NULL); query head h reads KV head h / (heads / kv_heads).  out: `dtype` [batch][seq][heads][dim],

@@ -352,7 +352,7 @@ __global__ void __launch_bounds__(C4_THREADS) cache4_load_kernel(const __grid_co
             const int at = n & 1 ? 8 : 0;
             const float2 c = make_float2(__uint_as_float((half & (15u << at)) | 0x4b000000u), __uint_as_float((half & (240u << at)) | 0x4b000000u));
             float2 y = __ffma2_rn(__fadd2_rn(c, back), step2[n & 1], m2);
-            if (PROMPT && sizeof(T) == 2 && !std::is_same<T, __nv_bfloat16>::value)  // (m + 15 s may lie a rounding above the largest float16)
+            if (std::is_same<T, __half>::value)  // (m + 15 s may lie a rounding above the largest float16)
                 y = make_float2(fminf(fmaxf(y.x, -C4_MOST), C4_MOST), fminf(fmaxf(y.y, -C4_MOST), C4_MOST));
             x[2 * n] = y.x;
             x[2 * n + 1] = y.y;

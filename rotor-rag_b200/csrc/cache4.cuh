@@ -126,6 +126,12 @@ __device__ __forceinline__ uint32_t pack_half(float lo, float hi) {
     const __half2 h = __floats2half2_rn(lo, hi);
     return *reinterpret_cast<const uint32_t*>(&h);
 }
+// The same for outputs of finite rows: what rounding takes above 65504 is that (NaN stays).
+__device__ __forceinline__ uint32_t pack_half_finite(float lo, float hi) {
+    uint32_t r;
+    asm("cvt.rn.satfinite.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+    return r;
+}
 __device__ __forceinline__ void store8(__half* p, const float (&x)[8]) {
     *reinterpret_cast<uint4*>(p) = make_uint4(pack_half(x[0], x[1]), pack_half(x[2], x[3]), pack_half(x[4], x[5]), pack_half(x[6], x[7]));
 }

@@ -172,7 +172,7 @@ __device__ __forceinline__ void store4(void* out, int dtype, size_t at, float4 y
     } else if (dtype == ROTOR_B200_BF16) {
         *reinterpret_cast<uint2*>(static_cast<__nv_bfloat16*>(out) + at) = float4_to_bf16x4(y);
     } else {
-        *reinterpret_cast<uint2*>(static_cast<__half*>(out) + at) = make_uint2(pack_half(y.x, y.y), pack_half(y.z, y.w));
+        *reinterpret_cast<uint2*>(static_cast<__half*>(out) + at) = make_uint2(pack_half_finite(y.x, y.y), pack_half_finite(y.z, y.w));
     }
 }
 

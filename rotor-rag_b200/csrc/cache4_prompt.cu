@@ -234,7 +234,10 @@ cache4_prompt_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_cons
                     for (int i = 0; i < 32; i += 16) {
                         uint32_t v[8];
 #pragma unroll
-                        for (int n = 0; n < 8; ++n) v[n] = p4_pack<HALF>(__uint_as_float(o[i + 2 * n]) * inv, __uint_as_float(o[i + 2 * n + 1]) * inv);
+                        for (int n = 0; n < 8; ++n) {
+                            const float a = __uint_as_float(o[i + 2 * n]) * inv, c = __uint_as_float(o[i + 2 * n + 1]) * inv;
+                            v[n] = HALF ? pack_half_finite(a, c) : t5_pack(a, c);
+                        }
                         if (p.whole) {
                             asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(out + c + i), "r"(v[0]), "r"(v[1]), "r"(v[2]),
                                          "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7])

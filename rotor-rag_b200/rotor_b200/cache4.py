@@ -100,7 +100,8 @@ class Cache4:
                 check(status, "cache4_append")
 
     def read(self, begin: int, end: int, dtype=None):
-        """What positions begin .. end - 1 stand for: keys and values [batch, kv_heads, end - begin, dim] (float32 unless told)."""
+        """What positions begin .. end - 1 stand for: keys and values [batch, kv_heads, end - begin, dim] (float32 unless told).
+        float16 holds 65504 where a code stands for a little more."""
         _, stream = self._here()
         dtype = dtype or abi._torch.float32
         if not 0 <= begin <= end <= self.max_seq:

@@ -139,3 +139,29 @@ def test_magnitudes_above_the_largest_float16(torch):
             k, v = cache.read(0, 16)
             want = held(t).astype(np.float32).astype(np.float64)
             assert np.array_equal(host(k), want) and np.array_equal(host(v), want[:, :, ::-1])
+
+
+@pytest.mark.parametrize("seq", [1, 300])
+def test_finite_float16_rows_stay_finite(torch, seq):
+    """From a step of 4096 on m + 15 s can lie above the largest float16: it is read as that, and weighted sums end there too."""
+    from rotor_b200.cache4 import Cache4
+    rng = np.random.default_rng(24)
+    batch, kv, dim, total = 8, 2, 64, 400
+    x = rng.uniform(-65504, 65504, (batch, total, kv, dim))
+    x[..., 0] = x[..., 32] = 65504
+    x[..., 1], x[..., 33] = rng.uniform(-65504, -1000, (2, batch, total, kv))
+    t = torch.from_numpy(x).cuda().half()
+    assert t.isfinite().all()
+    cache = Cache4(batch, kv, total, dim)
+    cache.append(t, t, 0)
+    want = held(t)
+    assert want.max() > 65520
+    k, v = cache.read(0, total, torch.float16)
+    assert np.array_equal(host(k), dense(torch, want, "float16")) and torch.equal(k, v)
+    assert host(cache.read(0, total)[0]).max() > 65520      # (float32 holds what the codes stand for)
+    q = torch.zeros((batch, seq, 4, dim), device="cuda", dtype=torch.float16)
+    out = cache.attend(q, total - seq, window=1)            # every row's own position
+    assert out.isfinite().all()
+    own = np.repeat(want[:, :, total - seq:].transpose(0, 2, 1, 3), 2, 2)
+    # 2^-11 for the weight, of |v| and of s code, and the output's half step
+    assert np.all(np.abs(host(out) - np.clip(own, -65504, 65504)) <= 2.0 ** -11 * (np.abs(own) + 2 * 65504 + 32) + 2.0 ** -11 * np.abs(own))
