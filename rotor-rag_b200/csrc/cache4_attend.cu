@@ -8,7 +8,12 @@
 // two of them; in the next four bits it is code 2^-20.  No code is converted, and nothing of a cached row is rounded.  The queries of
 // 16-bit types are exact in the other operand (a row is scaled by a power of two into float16's range; columns whose codes lie four bits
 // higher by another 1/16), float32 queries are split into two terms (2^-22 of the value).  The weights p_j are rounded to float16 and so
-// are their products with s_jg (2^-12 each; the sum of weights takes them as rounded), in float32 calls both are two terms (2^-22).
+// are their products with s_jg (2^-11 each, or 2^-25 where that is more, the largest weight of a row being 2^7 or more; the sum of weights
+// takes them as rounded).  In float32 calls both are two terms, the second held 2^10 times as large and with sums of its own, so that it keeps
+// its bits where the first is near float16's smallest numbers: 2^-22 of a weight, and 2^-35 of the largest.  There a warp multiplies s by a
+// power of two that takes the largest it has seen to between 2^-4 and 2, so that products keep these bits at values of any size.  (One sum for
+// both terms was off by up to 7e-4 for values of 1e-5, and took 58.5 us where this takes 65: 64 sequences behind 1024 .. 4095 positions, 64/8
+// heads of 128.)
 // Scores, maxima, sums and outputs are float32.  Matrix instructions cut their sums off instead of rounding them, which shows after many
 // of them in a row, and align their products as if a subnormal number had the smallest normal exponent: with codes in the lowest four bits
 // a sum is off by 1.7e-7 of its terms' size, four bits higher by 3e-9 (as with the codes as normal numbers).  float32 calls begin every
@@ -27,9 +32,10 @@
 
 namespace rb {
 
-constexpr float A4_SLACK = 7.f;   // a new maximum below the old one plus this (in powers of two) leaves the shift where it is
-constexpr float A4_LIFT = 7.f;    // weights are at most 2^(lift + slack): p s below 2^15 for s below 2, and a smaller lift for larger s
-constexpr float A4_LOW = -1e30f;  // a shift that any score is above
+constexpr float A4_LOW = -1e30f;     // a shift that any score is above
+constexpr float A4_SECOND = 1024.f;  // second terms of weights are held this many times as large
+constexpr int A4_MOST_UP = 14;       // with two terms s is multiplied by up to 2^14
+constexpr int A4_NEAR_ONE = 4;       // ... and by none where the largest is between 2^-4 and 2, as it is for values around 1
 constexpr int A4_JOIN = 256;      // threads of the join
 constexpr int A4_SORTED = 128;    // most sequences that are taken by their length
 constexpr int A4_CLUSTER = 8;     // most splits that are joined inside a cluster
@@ -99,6 +105,7 @@ __device__ __forceinline__ uint32_t turned(uint32_t v) {  // the 8 x 8 matrix of
     asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));
     return r;
 }
+__device__ __forceinline__ float two_to(int e) { return __int_as_float((127 + e) << 23); }
 __device__ __forceinline__ __half2 as_half2(uint32_t v) { return *reinterpret_cast<const __half2*>(&v); }
 __device__ __forceinline__ uint32_t as_word(__half2 v) { return *reinterpret_cast<const uint32_t*>(&v); }
 
@@ -192,6 +199,9 @@ template <int NG, int R, int TERMS, int W>
 __global__ void __launch_bounds__(32 * W, (NG * R <= 4 ? 16 : 8) / W) attend4_kernel(const __grid_constant__ Attend4 p) {
     using C = A4Cfg<NG, R, TERMS, W>;
     constexpr bool EXACT = TERMS > 1;
+    // A new maximum below the old one plus SLACK (powers of two) leaves the shift where it is, and weights are at most 2^(lift + SLACK).  p s is
+    // below 2^15 for s below 2, and for larger s the lift is smaller; with two terms p s is below 2^5, so that 2^10 times that is a float16 too.
+    constexpr float SLACK = EXACT ? 4.f : 7.f, LIFT = EXACT ? 0.f : 7.f;
     constexpr int THREADS = 32 * W, OWN = (NG + W - 1) / W;  // groups whose query operands a warp makes
     using T = Tile4<NG>;
     constexpr int D = C::D, Q = C::Q, S = C::STAGES;
@@ -343,7 +353,8 @@ __global__ void __launch_bounds__(32 * W, (NG * R <= 4 ? 16 : 8) / W) attend4_ke
     };
 
     float shift[R][2], o[R][2 * NG][4], rest[R][4];  // rest: row g: sum of p m of group g; row 8 (lanes 0 .. 3): sum of p
-    float lift = A4_LIFT;
+    float lift = LIFT;
+    float up = (float)(1 << A4_MOST_UP);  // EXACT: what s is multiplied by, a power of two; the sums o are that many times as large
 #pragma unroll
     for (int h = 0; h < R; ++h) {
         shift[h][0] = shift[h][1] = A4_LOW;
@@ -354,9 +365,10 @@ __global__ void __launch_bounds__(32 * W, (NG * R <= 4 ? 16 : 8) / W) attend4_ke
             for (int i = 0; i < 2 * NG; ++i) o[h][i][n] = 0.f;
         }
     }
-    auto rescale = [&](int h, float a0, float a1) {
+    auto rescale = [&](int h, float a0, float a1, float f) {
+        const float f0 = EXACT ? a0 * f : a0, f1 = EXACT ? a1 * f : a1;
 #pragma unroll
-        for (int i = 0; i < 2 * NG; ++i) o[h][i][0] *= a0, o[h][i][1] *= a1, o[h][i][2] *= a0, o[h][i][3] *= a1;
+        for (int i = 0; i < 2 * NG; ++i) o[h][i][0] *= f0, o[h][i][1] *= f1, o[h][i][2] *= f0, o[h][i][3] *= f1;
         rest[h][0] *= a0, rest[h][1] *= a1, rest[h][2] *= a0, rest[h][3] *= a1;
     };
     const int key_row = 4 * (g >> 1) + (g & 1);  // rows g and g + 8 of the key operand: this position of the tile, and two more
@@ -427,7 +439,7 @@ __global__ void __launch_bounds__(32 * W, (NG * R <= 4 ? 16 : 8) / W) attend4_ke
 #pragma unroll
             for (int i = 0; i < 4; ++i) sc[h][i] *= fa[h][i & 1];
 
-        // ---- the values' s; above 2 (bit 14 of a float16) the weights have to be kept smaller
+        // ---- the values' s; where one is 2 or more (bit 14 of a float16) weights, or with two terms s, have to be smaller
         Bytes<8 * NG> vs;
         vs.load(x + T::VS + t * (8 * NG));
         if (tile < inner0 || tile >= inner1) {
@@ -449,21 +461,37 @@ __global__ void __launch_bounds__(32 * W, (NG * R <= 4 ? 16 : 8) / W) attend4_ke
             }
         }
         uint32_t any = 0;
+        if constexpr (EXACT) {
+            // the largest, in both halves of the word (s is no negative number: floats in the order of their bits)
+            uint32_t most = 0u;
 #pragma unroll
-        for (int i = 0; i < 2 * NG; ++i) any |= vs.w[i];
+            for (int i = 0; i < 2 * NG; ++i) most = __vmaxu2(most, vs.w[i]);
+            any = as_word(__hmul2(as_half2(most), __float2half2_rn(up)));
+        } else {
+#pragma unroll
+            for (int i = 0; i < 2 * NG; ++i) any |= vs.w[i];
+        }
         bool higher = false;
 #pragma unroll
         for (int h = 0; h < R; ++h)
 #pragma unroll
-            for (int e = 0; e < 2; ++e) higher |= fmaxf(sc[h][e], sc[h][e + 2]) > shift[h][e] + (A4_SLACK + lift);
+            for (int e = 0; e < 2; ++e) higher |= fmaxf(sc[h][e], sc[h][e + 2]) > shift[h][e] + (SLACK + lift);
         if (__any_sync(0xffffffffu, higher || (any & 0x40004000u))) {
             float most = 0.f;
 #pragma unroll
             for (int i = 0; i < 4 * NG; ++i) most = fmaxf(most, vs.half_at(i));
             most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 1));
             most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 2));
-            const int exponent = (__float_as_int(most) >> 23) - 127;
-            const float now = fminf(lift, A4_LIFT - (float)max(exponent, 0));
+            const int exponent = (__float_as_int(most) >> 23) - 127;  // (of zero: -127)
+            const float now = EXACT ? lift : fminf(lift, LIFT - (float)max(exponent, 0));
+            float f = 1.f;
+            if constexpr (EXACT) {
+                const float best = two_to(exponent >= -A4_NEAR_ONE && exponent <= 0 ? 0 : min(-exponent, A4_MOST_UP));
+                if (best < up) {
+                    f = best * two_to(127 - (__float_as_int(up) >> 23));
+                    up = best;
+                }
+            }
 #pragma unroll
             for (int h = 0; h < R; ++h) {
                 float alpha[2];
@@ -476,9 +504,16 @@ __global__ void __launch_bounds__(32 * W, (NG * R <= 4 ? 16 : 8) / W) attend4_ke
                     alpha[e] = fast_exp2(shift[h][e] - m);
                     shift[h][e] = m;
                 }
-                rescale(h, alpha[0], alpha[1]);
+                rescale(h, alpha[0], alpha[1], f);
             }
             lift = now;
+        }
+        if constexpr (EXACT) {
+            if (up != 1.f) {
+                const __half2 f = __float2half2_rn(up);
+#pragma unroll
+                for (int i = 0; i < 2 * NG; ++i) vs.w[i] = as_word(__hmul2(as_half2(vs.w[i]), f));
+            }
         }
 
         // ---- weights, turned into the operand of the second product: row g of the queries, positions 4 t .. 4 t + 3
@@ -492,7 +527,7 @@ __global__ void __launch_bounds__(32 * W, (NG * R <= 4 ? 16 : 8) / W) attend4_ke
                 pw[h][0][u] = turned(w);
                 if (TERMS > 1) {
                     const float2 f = half2_of(w);
-                    pw[h][TERMS - 1][u] = turned(pack_half(e0 - f.x, e1 - f.y));
+                    pw[h][TERMS - 1][u] = turned(pack_half((e0 - f.x) * A4_SECOND, (e1 - f.y) * A4_SECOND));
                 }
             }
         }
@@ -505,12 +540,12 @@ __global__ void __launch_bounds__(32 * W, (NG * R <= 4 ? 16 : 8) / W) attend4_ke
             const uint32_t ones = g == 0 ? 0x3c003c00u : 0u;
 #pragma unroll
             for (int h = 0; h < R; ++h) {
-                float d[4] = {0.f, 0.f, 0.f, 0.f};
                 if constexpr (TERMS > 1) {
-                    a4_mma(d, vm.w[0], ones, vm.w[1], ones, pw[h][1][0], pw[h][1][1]);
+                    float d[4] = {0.f, 0.f, 0.f, 0.f}, l[4] = {0.f, 0.f, 0.f, 0.f};
+                    a4_mma(l, vm.w[0], ones, vm.w[1], ones, pw[h][1][0], pw[h][1][1]);
                     a4_mma(d, vm.w[0], ones, vm.w[1], ones, pw[h][0][0], pw[h][0][1]);
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) rest[h][i] += d[i];
+                    for (int i = 0; i < 4; ++i) rest[h][i] += fmaf(l[i], 1.f / A4_SECOND, d[i]);
                 } else {
                     a4_mma(rest[h], vm.w[0], ones, vm.w[1], ones, pw[h][0][0], pw[h][0][1]);
                 }
@@ -526,15 +561,23 @@ __global__ void __launch_bounds__(32 * W, (NG * R <= 4 ? 16 : 8) / W) attend4_ke
                 const __half2 s0 = as_half2(vs.w[2 * j]), s1 = as_half2(vs.w[2 * j + 1]);
                 const __half2 w0 = __hmul2(as_half2(pw[h][0][0]), s0), w1 = __hmul2(as_half2(pw[h][0][1]), s1);
                 if constexpr (TERMS > 1) {
-                    // what the rounding of p s left out, and the second term of p
-                    const __half2 l0 = __hfma2(as_half2(pw[h][1][0]), s0, __hfma2(as_half2(pw[h][0][0]), s0, __hneg2(w0)));
-                    const __half2 l1 = __hfma2(as_half2(pw[h][1][1]), s1, __hfma2(as_half2(pw[h][0][1]), s1, __hneg2(w1)));
+                    // the second term holds what the rounding of p s left out, and the second term of p
+                    const __half2 many = __float2half2_rn(A4_SECOND), t0 = __hmul2(s0, many), t1 = __hmul2(s1, many);
+                    const __half2 l0 = __hfma2(as_half2(pw[h][1][0]), s0, __hfma2(as_half2(pw[h][0][0]), t0, __hneg2(__hmul2(w0, many))));
+                    const __half2 l1 = __hfma2(as_half2(pw[h][1][1]), s1, __hfma2(as_half2(pw[h][0][1]), t1, __hneg2(__hmul2(w1, many))));
                     float d[4] = {0.f, 0.f, 0.f, 0.f}, d2[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
                     for (int term = 1; term >= 0; --term) {
                         const uint32_t b0 = as_word(term ? l0 : w0), b1 = as_word(term ? l1 : w1);
                         a4_mma(d, codes_of<EXACT, 0>(a), codes_of<EXACT, 1>(a), codes_of<EXACT, 0>(c), codes_of<EXACT, 1>(c), b0, b1);
                         a4_mma(d2, codes_of<EXACT, 2>(a), codes_of<EXACT, 3>(a), codes_of<EXACT, 2>(c), codes_of<EXACT, 3>(c), b0, b1);
+                        if (term) {
+#pragma unroll
+                            for (int i = 0; i < 4; ++i) {
+                                d[i] *= 1.f / A4_SECOND;
+                                d2[i] *= 1.f / A4_SECOND;
+                            }
+                        }
                     }
 #pragma unroll
                     for (int i = 0; i < 4; ++i) {
@@ -556,6 +599,7 @@ __global__ void __launch_bounds__(32 * W, (NG * R <= 4 ? 16 : 8) / W) attend4_ke
     float* all = reinterpret_cast<float*>(a4_raw + C::O);  // [warp][row][OS]
     float(*shifts)[Q] = reinterpret_cast<float(*)[Q]>(a4_raw + C::SHIFT);
     float(*masses)[Q] = reinterpret_cast<float(*)[Q]>(a4_raw + C::MASS);
+    const float down = two_to(127 - (__float_as_int(up) >> 23));
 #pragma unroll
     for (int h = 0; h < R; ++h) {
         const int r = 8 * h + 2 * t;
@@ -570,7 +614,7 @@ __global__ void __launch_bounds__(32 * W, (NG * R <= 4 ? 16 : 8) / W) attend4_ke
         for (int j = 0; j < NG; ++j) {
             // columns 32 j + 4 g .. + 3
             const float l0 = __shfl_sync(0xffffffffu, rest[h][0], 4 * j + t), l1 = __shfl_sync(0xffffffffu, rest[h][1], 4 * j + t);
-            constexpr float c0 = EXACT ? A4_HIGH_CODE : A4_LOW_CODE, c1 = A4_HIGH_CODE;
+            const float c0 = EXACT ? A4_HIGH_CODE * down : A4_LOW_CODE, c1 = EXACT ? A4_HIGH_CODE * down : A4_HIGH_CODE;
             const float(&a)[4] = o[h][2 * j], (&c)[4] = o[h][2 * j + 1];
             *reinterpret_cast<float4*>(to + 32 * j) = make_float4(fmaf(a[0], c0, l0), fmaf(a[2], c1, l0), fmaf(c[0], c0, l0), fmaf(c[2], c1, l0));
             *reinterpret_cast<float4*>(to + C::OS + 32 * j) =

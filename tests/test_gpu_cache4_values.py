@@ -119,6 +119,57 @@ def test_portions_over_the_codes(torch, seq, heads, kv, dim, past, kw, dtype):
     assert (np.abs(want) > bound).mean() > 0.9
 
 
+@pytest.mark.parametrize("dim", [64, 128, 192])
+@pytest.mark.parametrize("seq", [1, 20])
+@pytest.mark.parametrize("size", [1.0, 1e-2, 1e-3, 1e-4, 1e-5, "mixed", "mixed rows", 3000.0])
+def test_float32_weights_at_values_of_any_size(torch, size, seq, dim):
+    """The queries are short, so that what the scores' sums leave does not hide what the weights' two terms leave: a score is off by
+    2^-19 of the sum of |q| |k| (four additions of a group, its scaling, up to six groups, 2^-23 each; queries as two terms, 2^-22) and by the
+    exponential (its argument, up to 16, 2^-21; its result, 2^-22): 2^-20, twice with the ratio to the sum.  Weights as two terms, alone and times s,
+    are off by 2^-22 each, 2^-20 with the ratio; sums over the positions add 2^-23 a tile.  2^-17 of the weighted sums of |v| and of s code
+    holds all of them.  ("mixed": groups of 1, 1e-2, 1e-4 and 1 in turn, "mixed rows": the positions.)"""
+    from rotor_b200.cache4 import Cache4
+    rng = np.random.default_rng(21)
+    batch, heads, kv, past = 2, 8, 2, 150
+    total = past + seq
+    cache = Cache4(batch, kv, total, dim)
+    sizes = np.array([1.0, 1e-2, 1e-4, 1.0])
+    factor = np.repeat(sizes[np.arange(dim // 32) % 4], 32) if size == "mixed" else sizes[np.arange(total) % 4][:, None, None] if size == "mixed rows" else size
+    k = rows(torch, rng, (batch, total, kv, dim), "float32")
+    v = torch.from_numpy((rng.standard_normal((batch, total, kv, dim)) * factor).astype(np.float32)).cuda()
+    cache.append(k, v, 0)
+    q = torch.from_numpy((rng.standard_normal((batch, seq, heads, dim)) * 0.02).astype(np.float32)).cuda()
+    got = host(cache.attend(q, past, scale=dim ** -0.5))
+    want, weighted, reach = O.attend(host(q), held(k), held(v), [past] * batch, dim ** -0.5, 0, None, O.coded(host(v)).transpose(0, 2, 1, 3))
+    assert reach.max() < 1.0
+    err, bound = np.abs(got - want), 2.0 ** -17 * weighted + 2.0 ** -24 * np.abs(want)
+    assert np.all(err <= bound), float((err / bound).max())
+
+
+@pytest.mark.parametrize("dtype", HALVES)
+@pytest.mark.parametrize("size", [1e-3, 1e-5, 1e-6, "mixed", "growing", 3000.0])
+def test_16_bit_calls_at_values_of_any_size(torch, size, dtype):
+    """Groups of one size, groups of several, and positions whose values grow by a power of two every few rows: 2^-11 of the weighted sums
+    as everywhere, and the type's own steps."""
+    from rotor_b200.cache4 import Cache4
+    rng = np.random.default_rng(22)
+    batch, heads, kv, past, dim = 2, 8, 2, 300, 128
+    for seq in (1, 4):
+        total = past + seq
+        cache = Cache4(batch, kv, total, dim)
+        factor = (np.repeat([1.0, 1e-2, 30.0, 1.0], 32) if size == "mixed" else 2.0 ** (np.arange(total) // 16 - 9.0)[:, None, None] if size == "growing"
+                  else size)
+        k = rows(torch, rng, (batch, total, kv, dim), "float32")
+        v = torch.from_numpy((rng.standard_normal((batch, total, kv, dim)) * factor).astype(np.float32)).cuda()
+        cache.append(k, v, 0)
+        q = torch.from_numpy(rng.standard_normal((batch, seq, heads, dim)).astype(np.float32)).cuda().to(getattr(torch, dtype))
+        got = cache.attend(q, past)
+        want, weighted, reach = O.attend(host(q), held(k), held(v), [past] * batch, dim ** -0.5, 0, None, O.coded(host(v)).transpose(0, 2, 1, 3))
+        bound = bound_of(torch, dtype, want, weighted, reach, 2.0 ** -11, total, 0.0, 0.0)
+        err = np.abs(host(got) - want)
+        assert np.all(err <= bound), (seq, float((err / bound).max()))
+
+
 def test_magnitudes_above_the_largest_float16(torch):
     """They are stored as 65504 is: where a group's smallest value rounds up, that is not the highest code."""
     from rotor_b200.cache4 import Cache4
