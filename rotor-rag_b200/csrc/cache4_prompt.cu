@@ -10,7 +10,7 @@
 // writes 128 weights back, half of them at a time, so that the sums over the first half start while the second is made; no row is exchanged
 // between threads.  While one block's scores become weights, the tensor cores work for the other, and while a block's outputs are read, its
 // next queries arrive.  Outputs stay in tensor memory: the reference that weights are relative to moves, and the sums are scaled, only where a
-// row's maximum has grown by more than 2^8 (weights are at most that, the sum of weights is float32).  Warp 0: TMA; warp 1: MMA issue, all of
+// row's maximum has grown by more than 2^8 (weights are at most that, in float16 2^15; the sum of weights is float32).  Warp 0: TMA; warp 1: MMA issue, all of
 // one thread and executed in the order of issue: the scores of a tile overwrite weights that an MMA issued before reads.  The eight warps take
 // registers that the other four give back (216 and 72 of 168 each at launch; with 40 for the four the thread that issues spilled, 2% of the
 // time).
@@ -22,8 +22,8 @@
 // polynomials in the FMA pipe (10%, 0%); steps of 64 keys with two score blocks in flight for each block (30%: twice the barriers); items in
 // the same order for every round of CTAs (8%); weights against the last reference with a look at their sum afterwards, without the tile's
 // maximum (4 to 9%).
-// Rounded to the 16-bit type, beside the outputs: keys and values as dense rows (the tensor cores' operands) and weights (at most 2^8, their
-// sum is of unrounded ones); scores, maxima, sums and outputs are float32.
+// Rounded to the 16-bit type, beside the outputs: keys and values as dense rows (the tensor cores' operands) and weights (their sum is
+// of unrounded ones); scores, maxima, sums and outputs are float32.
 // Waits are bounded; a wait that runs out records a code in the library status word, the CTA stops issuing work, frees its tensor memory
 // and returns.  No multicast, this GPU's memory only.
 #include <cstdlib>
@@ -35,7 +35,12 @@ namespace rb {
 
 constexpr int P4_ROWS = 128, P4_KEYS = 128, P4_THREADS = 384;
 constexpr int P4_SOFT_REGS = 216, P4_OTHER_REGS = 72, P4_REGS = 168;  // 2 x 128 x 216 + 128 x 72 = 384 x 168
+// The reference of a row's weights: its maximum less LIFT powers of two, kept while the maximum is below it plus LIFT and SLACK.  bf16 weights have
+// float32's range; float16 ones end at 2^15 with this, and the smallest are 2^-32 of the largest instead of 2^-25 (131072 positions at 2^-25.5
+// beside one of 2^0 are 0.3 % of the mass).
 constexpr float P4_SLACK = 8.f;
+template <bool HALF>
+constexpr float P4_LIFT = HALF ? 7.f : 0.f;
 
 template <int DK>
 struct P4Cfg {
@@ -167,9 +172,9 @@ cache4_prompt_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_cons
                     for (int c = 0; c < 4; ++c) top[c] = fmaxf(top[c], __uint_as_float(s[c][i]));
                 float m = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3]));
                 m = m == -INFINITY ? m : m * p.scale2;
-                const bool grown = m > ref + P4_SLACK;
+                const bool grown = m > ref + (P4_SLACK + P4_LIFT<HALF>);
                 if (__any_sync(0xffffffffu, grown)) {
-                    const float now = grown ? m : ref, alpha = grown ? fast_exp2(ref - now) : 1.f;
+                    const float now = grown ? m - P4_LIFT<HALF> : ref, alpha = grown ? fast_exp2(ref - now) : 1.f;
                     ref = now;
                     mass *= alpha;
                     if (j > 0) {  // (the first tile's sums begin at zero)

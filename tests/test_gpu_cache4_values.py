@@ -4,8 +4,8 @@ the roundings the prompt kernel states.
 Prompts on dense rows: keys and values are given to the oracle as the kernel has them, rounded through float32 to the type (float16: at most
 65504), so that what is left is
  * a score: products accumulated in float32 over at most 128 columns, 2^-17 of the sum of |q| |k| (and of one), twice with the ratio to the sum;
- * the weights' rounding to the type, h = finfo(type).eps / 2 of the weighted sum of |v|; float16 weights below 2^-14 are off by 2^-25:
-   2^-25 of the sum of |v| over the positions;
+ * the weights' rounding to the type, h = finfo(type).eps / 2 of the weighted sum of |v|; float16 weights below 2^-14 are off by 2^-25, where
+   the largest of a row is 2^7 at least: 2^-32 of the sum of |v| over the positions;
  * sums of n positions in float32, 16 at a time: n / 16 additions of 2^-22 at most of the weighted sum of |v|;
  * the output's rounding, h of it, and of the smallest normal number below that.
 Attention over the codes, 16-bit types: weights and their products with s are float16, 2^-11 with the ratio to the sum, of the weighted sums of
@@ -72,7 +72,7 @@ def prompt(torch, seed, dtype, batch, seq, heads, kv, dim, past, window=0, sinks
     use = dim ** -0.5 if scale is None else scale
     args = past, use, window, None if s is None else host(s)
     want, size, reach = O.attend(host(q), kd, vd, *args)
-    bound = bound_of(torch, dtype, want, size, reach, torch.finfo(getattr(torch, dtype)).eps / 2, total, np.abs(vd).sum(2).max(), 2.0 ** -25)
+    bound = bound_of(torch, dtype, want, size, reach, torch.finfo(getattr(torch, dtype)).eps / 2, total, np.abs(vd).sum(2).max(), 2.0 ** -32)
     return got, want, bound, (host(q), kd, vd, args)
 
 
@@ -117,6 +117,38 @@ def test_portions_over_the_codes(torch, seq, heads, kv, dim, past, kw, dtype):
     err = np.abs(host(got) - want)
     assert np.all(err <= bound), float((err / bound).max())
     assert (np.abs(want) > bound).mean() > 0.9
+
+
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16", "float16"])
+@pytest.mark.parametrize("seq,batch", [(1, 1), (256, 8)])
+def test_one_position_outweighs_thousands(torch, seq, batch, dtype):
+    """One key is 2^25.5 times the others' weight and has values of zero: the outputs are what all the others give together.
+
+    Weights are off by 2^-32 of the largest (float16: half of 2^-24, the largest being 2^7 or more) or in float32 calls 2^-35 (half of 2^-24 in a
+    term held 2^10 times as large, the largest being 1 or more): times the sum of |v|, which is the others' number at most."""
+    from rotor_b200.cache4 import Cache4
+    past, kv, heads, dim = 6000, 1, 8, 64
+    total = past + seq
+    cache = Cache4(batch, kv, total, dim)
+    if seq > 1 and dtype != "float32":
+        assert needs(torch, cache, dtype, heads, seq, past) >= 4 * batch * kv * total * dim
+    k, v = torch.zeros((1, total, 1, dim), device="cuda"), torch.ones((1, total, 1, dim), device="cuda")
+    v[..., 1::2] = -0.5
+    k[0, 3, 0, 0], v[0, 3] = 15.0, 0.0
+    cache.append(k.expand(batch, -1, -1, -1), v.expand(batch, -1, -1, -1), 0)
+    q = torch.zeros((1, seq, heads, dim), device="cuda", dtype=getattr(torch, dtype))
+    q[..., 0] = 25.5 * np.log(2) / 15
+    got = host(cache.attend(q.expand(batch, -1, -1, -1), past, scale=1.0))
+    x = float(host(q[0, 0, 0, 0])) * 15
+    n = past + np.arange(seq)[:, None, None]                  # others that a row sees
+    share = n * np.exp(-x) / (1 + n * np.exp(-x))
+    want = share * O.held(host(v[0, 0, 0]))
+    half = torch.finfo(getattr(torch, dtype)).eps / 2
+    bound = np.abs(want) * (half + max(half, 2.0 ** -11) + np.expm1(2.0 ** -16 * (x + 1)) + total / 16 * 2.0 ** -22) + 2.0 ** -32 * n + half * 2.0 ** -14
+    if dtype == "float32":
+        bound = np.abs(want) * (half + 2.0 ** -21 + np.expm1(2.0 ** -16 * (x + 1)) + total / 16 * 2.0 ** -22) + 2.0 ** -35 * n
+    err = np.abs(got - want)
+    assert np.all(err <= bound), float((err / bound).max())
 
 
 @pytest.mark.parametrize("dim", [64, 128, 192])
