@@ -32,7 +32,7 @@
 
 namespace rb {
 
-constexpr float A4_LOW = -1e30f;     // a shift that any score is above
+constexpr float A4_LOW = -3.4028235e38f;  // the shift of rows that have seen nothing: no finite score is below
 constexpr float A4_SECOND = 1024.f;  // second terms of weights are held this many times as large
 constexpr int A4_MOST_UP = 14;       // with two terms s is multiplied by up to 2^14
 constexpr int A4_NEAR_ONE = 4;       // ... and by none where the largest is between 2^-4 and 2, as it is for values around 1

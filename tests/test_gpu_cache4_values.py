@@ -138,7 +138,7 @@ def test_one_position_outweighs_thousands(torch, seq, batch, dtype):
     cache.append(k.expand(batch, -1, -1, -1), v.expand(batch, -1, -1, -1), 0)
     q = torch.zeros((1, seq, heads, dim), device="cuda", dtype=getattr(torch, dtype))
     q[..., 0] = 25.5 * np.log(2) / 15
-    got = host(cache.attend(q.expand(batch, -1, -1, -1), past, scale=1.0))
+    got = host(cache.attend(q.repeat(batch, 1, 1, 1), past, scale=1.0))      # (rows that lie apart, as the prompt kernel asks)
     x = float(host(q[0, 0, 0, 0])) * 15
     n = past + np.arange(seq)[:, None, None]                  # others that a row sees
     share = n * np.exp(-x) / (1 + n * np.exp(-x))
@@ -248,3 +248,26 @@ def test_finite_float16_rows_stay_finite(torch, seq):
     own = np.repeat(want[:, :, total - seq:].transpose(0, 2, 1, 3), 2, 2)
     # 2^-11 for the weight, of |v| and of s code, and the output's half step
     assert np.all(np.abs(host(out) - np.clip(own, -65504, 65504)) <= 2.0 ** -11 * (np.abs(own) + 2 * 65504 + 32) + 2.0 ** -11 * np.abs(own))
+
+
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
+@pytest.mark.parametrize("seq", [1, 7, 300])
+def test_scores_of_any_size(torch, seq, dtype):
+    """Scores of 1e31 to 1e34, all below zero: the largest takes everything, as among small ones."""
+    from rotor_b200.cache4 import Cache4
+    rng = np.random.default_rng(25)
+    batch, kv, dim, total = 4, 2, 64, 350
+    k = torch.full((batch, total, kv, dim), 2.0, device="cuda")
+    best = torch.from_numpy(rng.integers(0, total - seq + 1, (batch, kv))).cuda()
+    for b in range(batch):
+        for h in range(kv):
+            k[b, best[b, h], h] = 1.0
+    v = rows(torch, rng, (batch, total, kv, dim), "float32")
+    cache = Cache4(batch, kv, total, dim)
+    cache.append(k, v, 0)
+    want = torch.stack([torch.stack([cache.read(0, total)[1][b, h, best[b, h]] for h in range(kv)]) for b in range(batch)])
+    for size in (1.0, 1e29, 1e31, 1e33):
+        got = cache.attend(torch.full((batch, seq, kv, dim), -size, device="cuda", dtype=getattr(torch, dtype)), total - seq, scale=10.0)
+        # one weight: 2^-11 with s, the value's and the output's rounding
+        bound = want.abs().double() * 2.0 ** -7 + (2.0 ** -10 if dtype != "float32" else 2.0 ** -20) * 8
+        assert ((got.double() - want[:, None].double()).abs() <= bound[:, None]).all(), size
