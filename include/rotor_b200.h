@@ -426,7 +426,8 @@ int rotor_b200_sample(const float* logits, int rows, int vocab, int mode, int to
  *    [groups][count].  workspace: 16-byte aligned, contents of no matter, rotor_b200_beam_select_workspace_bytes bytes; calls that use
  *    none (few logits) take NULL, and the others return ERR_WORKSPACE before anything is launched.
  *  reorder_states: row b * width + w of every state becomes what row b * width + beams[b][w] was, in place; rows whose beam is
- *    their own, or no index of the group, stay.  `states` is a HOST array, whose memory does not overlap; width <= 32. */
+ *    their own, or no index of the group, stay.  `states` is a HOST array, whose memory does not overlap; width <= 32.
+ *    A call that is refused has moved none of them. */
 #define ROTOR_B200_F32 0
 #define ROTOR_B200_BF16 1
 #define ROTOR_B200_F16 2

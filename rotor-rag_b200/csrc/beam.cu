@@ -538,6 +538,15 @@ __global__ void __launch_bounds__(REORDER_THREADS) reorder_kernel(const __grid_c
     }
 }
 
+// Bytes of a state's pieces, and how many a row has.
+static int state_unit(const rotor_b200_state& s) {
+    const uintptr_t all = (uintptr_t)s.data | s.row_stride | (s.segments > 1 ? s.segment_stride : 0) | s.segment_bytes;
+    int unit = 16;
+    while (all & (unit - 1)) unit >>= 1;
+    return unit;
+}
+static constexpr uint64_t STATE_UNITS = 0x7fffff00u;  // most pieces of a row
+
 // Parts of `rounds` rounds for at most `most` of them.
 static void beam_split(BeamSelect& p, int most) {
     const int all = (p.vocab + BEAM_ROUND - 1) / BEAM_ROUND, parts = most < all ? most : all;
@@ -712,6 +721,8 @@ int rotor_b200_reorder_states(const rotor_b200_state* states, int n, const int64
         for (int k = 0; k < i; ++k) RB_REQUIRE(states[k].data != s.data);  // (moved twice, by threads that do not wait for one another)
         RB_REQUIRE(groups * width == 1 || s.row_stride >= (size_t)(s.segments - 1) * s.segment_stride + s.segment_bytes);
     }
+    for (int i = 0; i < n; ++i)  // (a refused call has moved none of the states)
+        if (states[i].segment_bytes / state_unit(states[i]) > STATE_UNITS / states[i].segments) return ROTOR_B200_ERR_SHAPE;
     const cudaStream_t st = as_stream(stream);
     for (int begin = 0; begin < n;) {
         Reorder p;
@@ -722,11 +733,8 @@ int rotor_b200_reorder_states(const rotor_b200_state* states, int n, const int64
         for (; begin < n && p.n < REORDER_STATES; ++begin) {
             const rotor_b200_state& s = states[begin];
             if (s.segment_bytes == 0) continue;
-            const uintptr_t all = (uintptr_t)s.data | s.row_stride | (s.segments > 1 ? s.segment_stride : 0) | s.segment_bytes;
-            int unit = 16;
-            while (all & (unit - 1)) unit >>= 1;
+            const int unit = state_unit(s);
             const uint64_t per = s.segment_bytes / unit, units = per * s.segments;
-            if (units > 0x7fffff00u) return ROTOR_B200_ERR_SHAPE;
             const uint64_t more = (units + REORDER_THREADS - 1) / REORDER_THREADS;
             if (blocks + more > 0x7fffffffu) break;
             ReorderState& d = p.s[p.n++];
