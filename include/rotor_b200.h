@@ -417,7 +417,10 @@ int rotor_b200_sample(const float* logits, int rows, int vocab, int mode, int to
  * the vocabulary, and the states that follow.
  *  beam_select: a candidate is a token v after beam w of a group (the beams of one sequence), worth
  *    scores[w] + logits[w][v] - log(sum_u exp(logits[w][u])); out are the `count` best of each group, best first, of equal
- *    ones the lowest w, then the lowest v.  Values are compared in 64 bits and returned as float32.  `ended` (uint8
+ *    ones the lowest w, then the lowest v.  Values are added up and compared in 64 bits and returned as float32; the logarithm in
+ *    them is that of a float32 sum (off by up to 2e-7 as measured, by less than 2^-17 with up to 2^18 logits): candidates of
+ *    different beams that lie closer than that come in either order, the same one at every call; those of one beam are in the
+ *    order of their logits.  `ended` (uint8
  *    [groups][width] or NULL): a beam whose flag is set offers one candidate, (w, pad) with its score unchanged.  Logits that
  *    are -inf or NaN offer nothing, nor does a row that holds +inf or a beam whose score is not finite; where fewer than
  *    `count` candidates are left, the rest is filled with -inf and the lowest (w, v) that are not among them.

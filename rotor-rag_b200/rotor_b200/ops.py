@@ -202,7 +202,8 @@ def beam_select(logits, scores, count, ended=None, pad=0):
 
     ``logits`` [groups, width, vocab] (float32, bfloat16 or float16, tokens of a row side by side) after the beams, whose scores so
     far are ``scores`` float32 [groups, width]; a candidate is worth its beam's score plus the log-softmax of its logit.  Among equal
-    ones the lower beam, then the lower token comes first.  ``ended`` bool [groups, width]: such a beam offers itself alone, as
+    ones the lower beam, then the lower token comes first; candidates of different beams that lie closer than the float32 sum of a
+    row's exponentials is known (2e-7 of a score as measured) come in either order, the same one at every call.  ``ended`` bool [groups, width]: such a beam offers itself alone, as
     token ``pad`` with its score unchanged.  Logits of -inf or NaN, rows that hold +inf and beams whose score is not finite offer
     nothing; places that no candidate is left for hold -inf and the lowest unused (beam, token).  Up to 32 beams and 64 continuations."""
     device, stream = abi.device_and_stream()
