@@ -2,9 +2,9 @@
 // on the dense side and 80 in the cache.  A thread takes eight neighbouring columns of four positions (a multiple of four and the next
 // three): those are one word of each key row or two 8-byte words of a value tile, four threads are a group, and threads run along rows.
 // Four rows a thread keep enough loads in flight, and values leave in pieces of 8 bytes instead of 2.  Measured, 163840 rows of 128 columns
-// (2 x 8 x 2048 x 5): written from bf16 in 19.0 us (2.9 TB/s; bound by 19 instructions a column at 0.6 of the issue slots, and by how many warps
-// there are to fill them: with the columns as float32 in 62 registers 26, with eight rows a thread in 64 registers 26.7), from float32 in 18.1
-// (5.4 TB/s); read as bf16 in 9.6 us (5.7 TB/s), as float32 in 15.2 (6.4).
+// (2 x 8 x 2048 x 5): written from bf16 in 19.0 us (2.9 TB/s; latency: 19 instructions a column fill 0.6 of the issue slots, and
+// the warps that 48 registers leave room for not the rest: with the columns as float32 in 62 registers 26, with eight rows a thread in 64
+// registers 26.7), from float32 in 18.6 (5.2 TB/s); read as bf16 in 9.6 us (5.7 TB/s), as float32 in 15.2 (6.4).
 #include <type_traits>
 
 #include "cache4.cuh"

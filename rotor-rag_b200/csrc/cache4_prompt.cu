@@ -17,7 +17,8 @@
 // Bound: a tile of both blocks takes the tensor cores 2048 clocks and 3600 in all.  The chain of a block is weights (1900 clocks for 128 x 128:
 // 550 instructions a warp, and the other block's warps share the schedulers) -> sums -> next scores (1024 clocks of MMA, some 600 of barriers:
 // a barrier operation queues behind the special function unit's, 250 clocks).  Measured, bf16, 32 query and 8 KV heads of 128, causal, with the
-// dense rows made first: 8192 tokens of one sequence 508 us (1.08 PFLOP/s), 8 x 2048 tokens of 20 and 5 heads 190 us (0.91), float16 216.
+// dense rows made first: 8192 tokens of one sequence 501 us (1.10 PFLOP/s), 8 x 2048 tokens of 20 and 5 heads 184 to 190 us (0.92); float16
+// 186 to 207, most behind other work, so that the clock may be the reason (not looked into).
 // Tried and slower: outputs by 16 bytes (3%: halves of sectors); weights in one piece (3%); half or a quarter of the exponentials by
 // polynomials in the FMA pipe (10%, 0%); steps of 64 keys with two score blocks in flight for each block (30%: twice the barriers); items in
 // the same order for every round of CTAs (8%); weights against the last reference with a look at their sum afterwards, without the tile's

@@ -122,7 +122,10 @@ class Cache4:
         Query head h reads KV head h // (heads // kv_heads).  ``scale`` of the scores: 1 / sqrt(dim) unless given.  ``window`` > 0: a
         query sees that many positions, its own included.  ``sinks`` float32 [heads]: exp(sink) joins the softmax's denominator.
         ``longest``: with a tensor of lengths, the most that a sequence holds, by which the work is divided (the cache's size unless
-        given); longer lengths are taken as it.  A query that sees no position gives zeros."""
+        given); longer lengths are taken as it.  A query that sees no position gives zeros.
+
+        Prompts of 16-bit types run a kernel whose waits are bounded: after a synchronise ``abi.device_status()`` raises where one ran out
+        and left outputs unwritten."""
         device, stream = self._here()
         heads = q.shape[2] if q.dim() == 4 else 0
         seq, strides = self._rows("q", q, heads, device)
