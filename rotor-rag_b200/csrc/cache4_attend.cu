@@ -12,8 +12,8 @@
 // takes them as rounded).  In float32 calls both are two terms, the second held 2^10 times as large and with sums of its own, so that it keeps
 // its bits where the first is near float16's smallest numbers: 2^-22 of a weight, and 2^-35 of the largest.  There a warp multiplies s by a
 // power of two that takes the largest it has seen to between 2^-4 and 2, so that products keep these bits at values of any size.  (One sum for
-// both terms was off by up to 7e-4 for values of 1e-5, and took 58.5 us where this takes 65: 64 sequences behind 1024 .. 4095 positions, 64/8
-// heads of 128.)
+// both terms was off by 2e-5 of the weighted sums for values of 1e-5 and nearly equal scores, where this is within 2^-17, and took 58.5 us where
+// this takes 64.5: 64 sequences behind 1024 .. 4095 positions, 64/8 heads of 128.)
 // Scores, maxima, sums and outputs are float32.  Matrix instructions cut their sums off instead of rounding them, which shows after many
 // of them in a row, and align their products as if a subnormal number had the smallest normal exponent: with codes in the lowest four bits
 // a sum is off by 1.7e-7 of its terms' size, four bits higher by 3e-9 (as with the codes as normal numbers).  float32 calls begin every
